@@ -327,6 +327,74 @@ int ps_world_trajs(ps_engine* e, const float* center_to_world, float* out_dev);
 int32_t ps_num_agents(ps_engine* e);
 int32_t ps_num_map_tokens(ps_engine* e);
 
+/* ---- Fine-tuning operators ---------------------------------------------------------------------------------------------
+ * What turns scored rollouts (ps_pair_metric, ps_rollout_metric) into a step of the part that chose: the log-probability of a drawn
+ * choice (ps_set_mode_choice's table, or a token of a motion vocabulary), two losses over it, and the clipping of the gradients.  They need no
+ * engine: every pointer is a DEVICE pointer unless it says HOST, everything is enqueued on `stream` (a hipStream_t, NULL = the default
+ * stream; the stream's device must be the current one), nothing is synchronised, allocated or kept between calls, and every call can be
+ * captured into a graph.  Results depend on the inputs alone (no atomics): equal inputs give equal bits.  Workspaces belong to one call at
+ * a time, need no initialisation and are 8-byte aligned. */
+#define PS_F32 0
+#define PS_BF16 1
+#define PS_F16 2
+
+/* Rows of decisions: logits [rows] x [choices] of type `dtype`, row i at element i * row_stride (row_stride >= choices, any alignment the
+ * element type allows), choice [rows] (32- or 64-bit integers), mask [rows] uint8 or NULL (all valid).  Row order is the caller's: [replan][agent
+ * row], token positions ...  A masked row is not read (logits, choice and terms may hold anything there): its log-probability and its gradient
+ * are 0.  A valid row whose choice lies outside [0, choices), that holds a NaN or +inf, or only -inf, has log-probability and gradient NaN. */
+typedef struct ps_decisions {
+  const void* logits;
+  int64_t rows, choices, row_stride;
+  int32_t dtype, choice_bits;
+  const void* choice;
+  const uint8_t* mask;
+} ps_decisions;
+
+/* logp [rows] = logits[choice] - ln sum exp logits.  stat [rows][2] (or NULL) = (max, 1 / sum exp(logits - max)), what ps_choice_grad needs. */
+int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* stream);
+/* grad [rows][choices] (dense, of type dtype) = gain * coef[row] * (one-hot(choice) - softmax).  gain: one float or NULL (1).
+ * skip_if_one != 0: leave grad as it is when *gain == 1 (it already holds that result).  A row whose coef * gain is 0 gets zeros. */
+int ps_choice_grad(const ps_decisions* d, const float* coef, const float* stat, const float* gain, int32_t skip_if_one, void* grad, void* stream);
+
+/* The clipped policy loss with a KL term.  Per valid row, with logp as above, ratio = exp(logp - old_logp), d = ref_logp - logp:
+ *   -min(ratio * advantage, clip(ratio, 1 - clip_low, 1 + clip_high) * advantage) + kl_coef * (exp(d) - d - 1)
+ * summed, divided by the number of valid rows if `mean`, and multiplied by `scale`.  old_logp, advantage, ref_logp: float [rows]; ref_logp may
+ * be NULL when kl_coef is 0 (the reported KL is then 0).  No gradient flows to them. */
+typedef struct ps_policy_terms {
+  const float *old_logp, *advantage, *ref_logp;
+  double clip_low, clip_high, kl_coef, scale;
+  int32_t mean;
+} ps_policy_terms;
+int64_t ps_policy_loss_workspace(const ps_decisions* d);
+/* loss [1]; kl [1] = mean KL over the valid rows; clip_frac [1] = share of the valid rows whose ratio is held by the clipping; logp [rows];
+ * stat [rows][2] and coef [rows] = d loss / d logp (or NULL both) for a later ps_choice_grad; grad [rows][choices] = d loss / d logits (or NULL:
+ * the loss only).  No valid row: all three numbers are 0. */
+int ps_policy_loss(const ps_decisions* d, const ps_policy_terms* t, float* loss, float* kl, float* clip_frac, float* logp, float* stat, float* coef,
+                   void* grad, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The preference loss of pairs of rollouts: better / worse [pairs][steps] float log-probabilities of the choices (ps_choice_logp), *_ref the same
+ * under a reference policy (NULL: 0), *_mask uint8 or NULL.  h = sum(better - better_ref) - sum(worse - worse_ref) over the valid steps,
+ *   loss = scale * mean (or sum) over pairs of  -(1 - label_smoothing) ln sigmoid(beta h) - label_smoothing ln sigmoid(-beta h). */
+typedef struct ps_preference {
+  const float *better, *better_ref, *worse, *worse_ref;
+  const uint8_t *better_mask, *worse_mask;
+  int64_t pairs, better_steps, worse_steps;
+  double beta, label_smoothing, scale;
+  int32_t mean;
+} ps_preference;
+int64_t ps_preference_loss_workspace(int64_t pairs);
+/* loss [1]; margin [pairs] = beta h; coef [pairs] = d loss / d h, for ps_preference_grad. */
+int ps_preference_loss(const ps_preference* q, float* loss, float* margin, float* coef, void* workspace, int64_t workspace_bytes, void* stream);
+/* better_grad [pairs][better_steps] = gain * coef on the valid steps, worse_grad = -gain * coef; either may be NULL.  gain: one float. */
+int ps_preference_grad(const ps_preference* q, const float* coef, const float* gain, float* better_grad, float* worse_grad, void* stream);
+
+/* Gradient clipping by the global norm, in place: norm [1] = sqrt(sum of squares over all n tensors), and every element is multiplied by
+ * min(1, max_norm / (norm + eps)) (not touched when that is 1; max_norm = inf only measures; a NaN norm makes NaN gradients).  HOST tables:
+ * ptr [n] device pointers to dense tensors that do not overlap, numel [n], dtype [n] (PS_F32 ...); read before the call returns. */
+int64_t ps_clip_grads_workspace(int32_t n, const int64_t* numel);
+int ps_clip_grads(int32_t n, void* const* ptr, const int64_t* numel, const int32_t* dtype, double max_norm, double eps, float* norm,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Timing on the engine's own stream (HIP events): run `iters` rollouts after `warmup`, return
  * average ms per rollout in *ms_rollout and, if stage_ms != NULL, per-stage averages
  * [encode_scene, generate_policy, replan loop]. */

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -18,6 +19,7 @@
 #include "ps_attn.h"
 #include "ps_kernels.h"
 #include "ps_chain16.h"
+#include "ps_internal.h"
 #include "ps_pe_learn.h"
 #include "ps_rowtile.h"
 
@@ -47,6 +49,18 @@ static void warn_ignored_experiment_env() {
 extern "C" const char* ps_last_error(void) { return g_err.c_str(); }
 static int fail(int code, const std::string& msg) {
   g_err = msg;
+  return code;
+}
+int ps::set_error(int code, const char* fmt, ...) noexcept {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  try {
+    g_err = buf;
+  } catch (...) {   // (out of host memory: the code is all that can be said)
+  }
   return code;
 }
 #define HIPCHK(x)                                                                                  \
