@@ -350,8 +350,10 @@ typedef struct ps_decisions {
   const uint8_t* mask;
 } ps_decisions;
 
+/* Bytes of workspace ps_choice_logp and ps_policy_loss want for these rows. */
+int64_t ps_choice_workspace(const ps_decisions* d);
 /* logp [rows] = logits[choice] - ln sum exp logits.  stat [rows][2] (or NULL) = (max, 1 / sum exp(logits - max)), what ps_choice_grad needs. */
-int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* stream);
+int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* workspace, int64_t workspace_bytes, void* stream);
 /* grad [rows][choices] (dense, of type dtype) = gain * coef[row] * (one-hot(choice) - softmax).  gain: one float or NULL (1).
  * skip_if_one != 0: leave grad as it is when *gain == 1 (it already holds that result).  A row whose coef * gain is 0 gets zeros. */
 int ps_choice_grad(const ps_decisions* d, const float* coef, const float* stat, const float* gain, int32_t skip_if_one, void* grad, void* stream);
@@ -365,7 +367,6 @@ typedef struct ps_policy_terms {
   double clip_low, clip_high, kl_coef, scale;
   int32_t mean;
 } ps_policy_terms;
-int64_t ps_policy_loss_workspace(const ps_decisions* d);
 /* loss [1]; kl [1] = mean KL over the valid rows; clip_frac [1] = share of the valid rows whose ratio is held by the clipping; logp [rows];
  * stat [rows][2] and coef [rows] = d loss / d logp (or NULL both) for a later ps_choice_grad; grad [rows][choices] = d loss / d logits (or NULL:
  * the loss only).  No valid row: all three numbers are 0. */

@@ -25,9 +25,11 @@ typedef __bf16 bf16;
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }   // (round to nearest even, once per stored element)
 
-// e^d for d <= 0.  fp32 elements take the library's expf (their results keep 24 bits); 16-bit elements v_exp_f32 on d * log2(e): the
-// product's rounding is |d| 2^-24 relative, weighted by e^d <= 1, far under the 2^-9 / 2^-12 of the element's own type.
-template <typename T> __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f); }
+// e^d for d <= 0.  fp32 elements take the library's expf (their results keep 24 bits); 16-bit elements v_exp_f32 on d * log2(e), the constant
+// in two parts (in one, its error would move every term of a sum the same way): what is left is the product's rounding, |d| 2^-24 relative.
+template <typename T> __device__ __forceinline__ float exp_of(float d) {
+  return __builtin_amdgcn_exp2f(fmaf(d, 1.92596299e-8f, d * 1.44269502e+0f));
+}
 template <> __device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
 
 // ---- block reductions (fixed order) ----------------------------------------------------------------------------------------
@@ -101,106 +103,502 @@ __device__ __forceinline__ RowLoss row_loss(const Policy& p, int64_t i, double l
   }
   return o;
 }
-// scale / n of the loss: n = valid rows for the mean (an empty mask divides by 1: the sums are zero then), 1 for the sum
-__device__ __forceinline__ double row_weight(const Policy& p, int64_t rows) {
-  const int64_t n = p.mean ? (p.count ? *p.count : rows) : 1;
-  return p.scale / (double)(n > 0 ? n : 1);
+constexpr int LOGP = 0, POLICY = 1;
+constexpr int kMaxGrid = 2048;        // row blocks of a launch (8 per CU); rows are dealt out in turn
+constexpr int64_t kCountInline = 1024;   // masks up to this many rows are counted by every block itself, longer ones by a launch of their own
+
+// What a launch over rows reads and writes.
+struct RowIo {
+  Rows r;
+  Policy p;
+  float* logp;
+  float2* stat;         // (maximum, 1 / sum) per row, or NULL
+  float* coef;          // d loss / d logp per row, or NULL
+  void* dx;             // gradient, dense, or NULL
+  double* part;         // (loss, kl, clipped) per block
+  float *loss, *kl, *clip_frac;
+};
+
+// 16 bytes of a row, kept packed in registers.  Rows of odd length start at any element: gfx950 loads and stores 16 bytes at element alignment.
+template <typename T> struct Reg {
+  static constexpr int N = 16 / sizeof(T);
+  uint32_t w[4];
+  struct __attribute__((packed, aligned(sizeof(T)))) Mem { uint32_t w[4]; };
+  __device__ __forceinline__ void load(const T* p) {
+    const Mem m = *(const Mem*)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = m.w[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    Mem m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m.w[i] = w[i];
+    *(Mem*)p = m;
+  }
+  // the packed words are what lives from one use to the next: without this the compiler keeps the 32-bit elements of the first use (twice the
+  // registers, 128 - 2000 B of scratch per lane in the widest kernels)
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])); }
+  __device__ __forceinline__ void get(float* f) const;
+  __device__ __forceinline__ void set(const float* f);
+};
+template <> __device__ __forceinline__ void Reg<float>::get(float* f) const {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+}
+template <> __device__ __forceinline__ void Reg<float>::set(const float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
+}
+template <> __device__ __forceinline__ void Reg<bf16>::get(float* f) const {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  const T2 t = {from_f32<T>(a), from_f32<T>(b)};
+  uint32_t u;
+  __builtin_memcpy(&u, &t, 4);
+  return u;
+}
+template <> __device__ __forceinline__ void Reg<bf16>::set(const float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2<bf16>(f[2 * i], f[2 * i + 1]);
+}
+template <> __device__ __forceinline__ void Reg<f16>::get(float* f) const {
+  typedef f16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h2 h;
+    __builtin_memcpy(&h, &w[i], 4);
+    f[2 * i] = (float)h.x;
+    f[2 * i + 1] = (float)h.y;
+  }
+}
+template <> __device__ __forceinline__ void Reg<f16>::set(const float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2<f16>(f[2 * i], f[2 * i + 1]);
 }
 
-constexpr int LOGP = 0, POLICY = 1;
-constexpr int kRowThreads = 256;
-constexpr int kMaxGrid = 2048;        // row blocks of a launch (8 per CU); rows are dealt out in turn
+// (maximum, sum of exponentials relative to it) of a part of a row.  A part of -inf alone keeps the maximum -inf and the sum 0.
+struct Part { double s; float m; };
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
+// join the parts of a group of lanes (G a power of two); every lane gets the result
+template <int G> __device__ __forceinline__ Part join_lanes(Part a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  double s = a.s == 0.0 ? 0.0 : a.s * exp((double)a.m - (double)m);      // (NaN sums stay NaN: NaN == 0 is false)
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) s += __shfl_xor(s, o);
+  return Part{s, m};
+}
 
-// One block per row: maximum, sum of exponentials, then (GRAD) the gradient -- three passes over the row.
-template <typename T, int MODE, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads) k_rows(Rows r, Policy p, float* logp_out, float2* stat, float* coef_out, T* dx, double* part) {
-  __shared__ double sd[kRowThreads / 64];
-  __shared__ float sf[kRowThreads / 64];
-  double loss = 0.0, kl = 0.0, clip = 0.0;
-  for (int64_t i = blockIdx.x; i < r.rows; i += gridDim.x) {
-    const T* x = (const T*)r.x + i * r.stride;
-    if (r.mask && !r.mask[i]) {     // (uniform over the block) a masked row is not read: its logits may hold anything
-      if (threadIdx.x == 0) {
-        logp_out[i] = 0.0f;
-        if (stat) stat[i] = make_float2(0.0f, 0.0f);
-        if (MODE == POLICY && coef_out) coef_out[i] = 0.0f;
+__device__ __forceinline__ int nonzero_bytes(const Reg<uint8_t>& q) {
+  int c = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int b = 0; b < 32; b += 8) c += (q.w[i] >> b & 255u) != 0;
+  return c;
+}
+// The valid rows the mean divides by, as scale / n; `count` is filled for the epilogue.  Called by the whole block.
+template <int THREADS> __device__ __forceinline__ double weight_of(const RowIo& io, int64_t* count, double* sd) {
+  const Policy& p = io.p;
+  int64_t n = io.r.rows;
+  if (io.r.mask) {
+    if (p.count) {
+      n = *p.count;
+    } else {
+      const uint8_t* mask = io.r.mask;
+      int c = 0;
+      const int64_t full = io.r.rows / 16;
+      for (int64_t j = threadIdx.x; j < full; j += THREADS) {
+        Reg<uint8_t> q;
+        q.load(mask + j * 16);
+        c += nonzero_bytes(q);
       }
-      if (GRAD)
-        for (int64_t j = threadIdx.x; j < r.k; j += kRowThreads) dx[i * r.k + j] = from_f32<T>(0.0f);
-      continue;
-    }
-    float m = -INFINITY;
-    for (int64_t j = threadIdx.x; j < r.k; j += kRowThreads) m = fmaxf(m, to_f32(x[j]));
-    m = block_max<kRowThreads>(m, sf);
-    double s = 0.0;
-    for (int64_t j = threadIdx.x; j < r.k; j += kRowThreads) s += (double)exp_of<T>(to_f32(x[j]) - m);
-    s = block_sum<kRowThreads>(s, sd);
-    const int64_t c = choice_of(r, i);
-    const bool ok = c >= 0 && c < r.k;
-    const double logp = ok ? ((double)to_f32(x[ok ? c : 0]) - (double)m) - log(s) : (double)NAN;
-    const float inv = ok ? (float)(1.0 / s) : NAN;      // (a choice outside the row makes its gradient NaN too)
-    if (threadIdx.x == 0) {
-      logp_out[i] = (float)logp;
-      if (stat) stat[i] = make_float2(m, inv);
-    }
-    if (MODE == POLICY) {
-      const RowLoss o = row_loss(p, i, logp);
-      const float coef = (float)(o.d_logp * row_weight(p, r.rows));
-      if (threadIdx.x == 0) {
-        loss += o.loss;
-        kl += o.kl;
-        clip += o.clip;
-        if (coef_out) coef_out[i] = coef;
-      }
-      if (GRAD)
-        for (int64_t j = threadIdx.x; j < r.k; j += kRowThreads)
-          dx[i * r.k + j] = from_f32<T>(coef * ((j == c ? 1.0f : 0.0f) - exp_of<T>(to_f32(x[j]) - m) * inv));
+      if (threadIdx.x < 16 && full * 16 + threadIdx.x < io.r.rows) c += mask[full * 16 + threadIdx.x] != 0;
+      n = (int64_t)block_sum<THREADS>((double)c, sd);
     }
   }
-  if (MODE == POLICY && threadIdx.x == 0) {
-    part[blockIdx.x * 3 + 0] = loss;
-    part[blockIdx.x * 3 + 1] = kl;
-    part[blockIdx.x * 3 + 2] = clip;
+  *count = n;
+  return p.scale / (double)(p.mean && n > 0 ? n : 1);
+}
+// What a row's statistics make of it: log-probability, loss terms, the coefficient of its gradient.  Every lane of the row's group calls it.
+struct RowEnd { float coef, inv; };
+template <int MODE> __device__ __forceinline__ RowEnd end_row(const RowIo& io, int64_t i, int64_t c, bool ok, float xc, Part a, double weight, bool writer, double* acc) {
+  const double logp = ok ? ((double)xc - (double)a.m) - log(a.s) : (double)NAN;
+  RowEnd e;
+  e.inv = ok ? (float)(1.0 / a.s) : NAN;      // (a choice outside the row makes its gradient NaN too)
+  e.coef = 0.0f;
+  if (MODE == POLICY) {
+    const RowLoss o = row_loss(io.p, i, logp);
+    e.coef = (float)(o.d_logp * weight);
+    if (writer) {
+      acc[0] += o.loss;
+      acc[1] += o.kl;
+      acc[2] += o.clip;
+    }
+  }
+  if (writer) {
+    io.logp[i] = (float)logp;
+    if (io.stat) io.stat[i] = make_float2(a.m, e.inv);
+    if (MODE == POLICY && io.coef) io.coef[i] = e.coef;
+  }
+  return e;
+}
+__device__ __forceinline__ void masked_row(const RowIo& io, int64_t i) {
+  io.logp[i] = 0.0f;
+  if (io.stat) io.stat[i] = make_float2(0.0f, 0.0f);
+  if (io.coef) io.coef[i] = 0.0f;
+}
+// the block's share of the sums -- or, where the launch is one block, the results themselves
+template <int THREADS> __device__ __forceinline__ void end_block(const RowIo& io, int64_t block, const double* acc, int64_t count, double weight, double* sd) {
+  double v[3];
+  for (int q = 0; q < 3; ++q) v[q] = block_sum<THREADS>(acc[q], sd);
+  if (threadIdx.x) return;
+  if (gridDim.x > 1 || gridDim.y > 1) {
+    for (int q = 0; q < 3; ++q) io.part[block * 3 + q] = v[q];
+    return;
+  }
+  const double inv = 1.0 / (double)(count > 0 ? count : 1);
+  *io.loss = (float)(v[0] * weight);
+  *io.kl = (float)(v[1] * inv);
+  *io.clip_frac = (float)(v[2] * inv);
+}
+
+// Short rows: G lanes hold a row, N elements each.
+template <typename T, int G, int N, int MODE, bool GRAD> __global__ void __launch_bounds__(256) k_rows_short(RowIo io) {
+  __shared__ double sd[4];
+  double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
+  int64_t count = 0;
+  if (MODE == POLICY) weight = weight_of<256>(io, &count, sd);
+  const Rows& r = io.r;
+  const int lane = threadIdx.x & (G - 1), k = (int)r.k;
+  for (int64_t i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; i < r.rows; i += (int64_t)gridDim.x * (256 / G)) {
+    T* dx = GRAD ? (T*)io.dx + i * k : nullptr;
+    if (r.mask && !r.mask[i]) {
+      if (lane == 0) masked_row(io, i);
+      if (GRAD)
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+          if (q * G + lane < k) dx[q * G + lane] = from_f32<T>(0.0f);
+      continue;
+    }
+    const T* x = (const T*)r.x + i * r.stride;
+    const int64_t c = choice_of(r, i);
+    const bool ok = c >= 0 && c < k;
+    const float xc = to_f32(x[ok ? c : 0]);
+    float f[N];
+    Part a{0.0, -INFINITY};
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      f[q] = q * G + lane < k ? to_f32(x[q * G + lane]) : -INFINITY;
+      a.m = fmaxf(a.m, f[q]);
+    }
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) a.m = fmaxf(a.m, __shfl_xor(a.m, o));
+    const float base = base_of(a.m);
+    float t = 0.0f;
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      f[q] = exp_of<T>(f[q] - base);
+      t += f[q];
+    }
+    a.s = (double)t;
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) a.s += __shfl_xor(a.s, o);
+    const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, lane == 0, acc);
+    if (GRAD) {
+      const float scale = -e.coef * e.inv;
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        if (q * G + lane < k) dx[q * G + lane] = from_f32<T>(fmaf(f[q], scale, q * G + lane == c ? e.coef : 0.0f));
+    }
+  }
+  if (MODE == POLICY) end_block<256>(io, blockIdx.x, acc, count, weight, sd);
+}
+
+// one 16-byte piece of a row's gradient, -coef e^(x - m) inv; the chosen element's share of coef is added behind it (chosen_element)
+template <typename T> __device__ __forceinline__ void grad_piece(Reg<T>& v, float m, float scale) {
+  float f[Reg<T>::N];
+  v.get(f);
+#pragma unroll
+  for (int i = 0; i < Reg<T>::N; ++i) f[i] = exp_of<T>(f[i] - m) * scale;
+  v.set(f);
+}
+// Thread t of TPR owns the piece the chosen column c lies in (pieces of V elements dealt out in turn from column j0, a tail of single elements behind
+// the last whole one): it writes that element once more, whole.
+template <typename T, int TPR> __device__ __forceinline__ void chosen_element(T* dx, int64_t j0, int64_t j1, int64_t c, int t, float xc, float m, float scale, float coef) {
+  if (c < j0 || c >= j1) return;
+  const int64_t o = c - j0, n = (j1 - j0) / Reg<T>::N;
+  const int owner = o < n * Reg<T>::N ? (int)(o / Reg<T>::N % TPR) : (int)(o - n * Reg<T>::N);
+  if (t == owner) dx[c] = from_f32<T>(fmaf(exp_of<T>(xc - m), scale, coef));
+}
+template <typename T, int THREADS> __device__ __forceinline__ void zero_row(T* dx, int64_t k, int t) {
+  Reg<T> z;
+  z.w[0] = z.w[1] = z.w[2] = z.w[3] = 0;
+  const int64_t nv = k / Reg<T>::N;
+  for (int64_t q = t; q < nv; q += THREADS) z.store(dx + q * Reg<T>::N);
+  if (nv * Reg<T>::N + t < k && t < Reg<T>::N) dx[nv * Reg<T>::N + t] = from_f32<T>(0.0f);
+}
+
+// Rows that fit the registers of WAVES waves, NV 16-byte pieces per thread: one read of the row for its statistics and its gradient.  One row per
+// group of waves and no loop over rows: inside a loop the compiler would hold the 64-bit functions' constants in 40 registers all the time.
+template <typename T, int WAVES, int NV, int MODE, bool GRAD> __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) k_rows_held(RowIo io) {
+  constexpr int THREADS = WAVES == 1 ? 256 : WAVES * 64, TPR = WAVES * 64, V = Reg<T>::N;
+  __shared__ double sd[THREADS / 64];
+  __shared__ Part joined[WAVES];
+  const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (block * (THREADS / TPR) >= io.r.rows) return;      // (the last line of a two-dimensional grid)
+  double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
+  int64_t count = 0;
+  if (MODE == POLICY) weight = weight_of<THREADS>(io, &count, sd);
+  const Rows& r = io.r;
+  const int t = threadIdx.x % TPR, nv = (int)(r.k / V), rest = (int)(r.k - (int64_t)nv * V);
+  const int64_t i = block * (THREADS / TPR) + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);    // (a wave has one row: its addresses live in scalar registers)
+  if (i < r.rows) {
+    T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
+    if (r.mask && !r.mask[i]) {        // (uniform over the row's threads)
+      if (t == 0) masked_row(io, i);
+      if (GRAD) zero_row<T, TPR>(dx, r.k, t);
+    } else {
+      const T* x = (const T*)r.x + i * r.stride;
+      Reg<T> v[NV];
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (q * TPR + t < nv) v[q].load(x + q * (TPR * V) + (uint32_t)(t * V));
+      const int64_t tail = (int64_t)nv * V + t;
+      const float last = t < rest ? to_f32(x[tail]) : -INFINITY;
+      const int64_t c = choice_of(r, i);
+      const bool ok = c >= 0 && c < r.k;
+      const float xc = to_f32(x[ok ? c : 0]);
+      Part a{0.0, last};
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (q * TPR + t < nv) {
+          float f[V];
+          v[q].get(f);
+#pragma unroll
+          for (int j = 0; j < V; ++j) a.m = fmaxf(a.m, f[j]);
+        }
+      a.m = wave_max(a.m);
+      const float base = base_of(a.m);
+      a.s = (double)exp_of<T>(last - base);
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (q * TPR + t < nv) {
+          float f[V], e = 0.0f;
+          v[q].forget();
+          v[q].get(f);
+#pragma unroll
+          for (int j = 0; j < V; ++j) e += exp_of<T>(f[j] - base);
+          a.s += (double)e;          // (eight terms in 32 bits, then 64)
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      a.s = wave_sum(a.s);
+      if (WAVES > 1) {
+        const int lane = threadIdx.x & 63;
+        if (lane == 0) joined[threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = joined[lane & (WAVES - 1)];
+        a = join_lanes<WAVES>(a);
+      }
+      const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, t == 0, acc);
+      if (GRAD) {
+        const float scale = -e.coef * e.inv;
+#pragma unroll
+        for (int q = 0; q < NV; ++q)
+          if (q * TPR + t < nv) {
+            v[q].forget();
+            grad_piece<T>(v[q], a.m, scale);
+            v[q].store(dx + q * (TPR * V) + (uint32_t)(t * V));
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        if (t < rest) dx[tail] = from_f32<T>(exp_of<T>(last - a.m) * scale);
+        if (ok) chosen_element<T, TPR>(dx, 0, r.k, c, t, xc, a.m, scale, e.coef);
+      }
+    }
+  }
+  if (MODE == POLICY) end_block<THREADS>(io, block, acc, count, weight, sd);
+}
+
+// (maximum, sum) of the elements [j0, j1) of a row by one block, in one pass: every thread keeps its running maximum and rescales its sum when it
+// grows.  j0 is a multiple of 16 bytes' worth of elements; THREADS a power of two of waves.
+template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(const T* x, int64_t j0, int64_t j1, Part* slots) {
+  constexpr int V = Reg<T>::N;
+  Part a{0.0, -INFINITY};
+  const int64_t n = (j1 - j0) / V;
+  auto take = [&](const float* f, int cnt) {
+    float m = f[0];
+    for (int j = 1; j < cnt; ++j) m = fmaxf(m, f[j]);
+    if (m > a.m) {
+      if (a.s != 0.0) a.s *= (double)exp_of<T>(a.m - m);      // (nothing yet, or -inf alone: 0 stays 0)
+      a.m = m;
+    }
+    const float base = base_of(a.m);
+    float e = 0.0f;
+    for (int j = 0; j < cnt; ++j) e += exp_of<T>(f[j] - base);
+    a.s += (double)e;
+  };
+  for (int64_t q = threadIdx.x; q < n; q += THREADS) {
+    Reg<T> v;
+    v.load(x + j0 + q * V);
+    float f[V];
+    v.get(f);
+    take(f, V);
+  }
+  const int64_t tail = j0 + n * V + threadIdx.x;
+  if (tail < j1) {
+    const float f = to_f32(x[tail]);
+    take(&f, 1);
+  }
+  a = join_lanes<64>(a);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = a;
+  __syncthreads();
+  a = slots[threadIdx.x & (THREADS / 64 - 1)];
+  return join_lanes<THREADS / 64>(a);
+}
+template <typename T, int THREADS> __device__ __forceinline__ void stream_grad(const T* x, T* dx, int64_t j0, int64_t j1, float m, float scale, float coef, int64_t c, float xc) {
+  constexpr int V = Reg<T>::N;
+  const int64_t n = (j1 - j0) / V;
+  for (int64_t q = threadIdx.x; q < n; q += THREADS) {
+    Reg<T> v;
+    v.load(x + j0 + q * V);
+    grad_piece<T>(v, m, scale);
+    v.store(dx + j0 + q * V);
+  }
+  const int64_t tail = j0 + n * V + threadIdx.x;
+  if (tail < j1) dx[tail] = from_f32<T>(exp_of<T>(to_f32(x[tail]) - m) * scale);
+  chosen_element<T, THREADS>(dx, j0, j1, c, threadIdx.x, xc, m, scale, coef);
+}
+
+// Rows longer than the registers of a block: a pass for the statistics, a second one for the gradient.
+template <typename T, int MODE, bool GRAD> __global__ void __launch_bounds__(1024) k_rows_long(RowIo io) {
+  __shared__ double sd[16];
+  __shared__ Part slots[16];
+  double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
+  int64_t count = 0;
+  if (MODE == POLICY) weight = weight_of<1024>(io, &count, sd);
+  const Rows& r = io.r;
+  for (int64_t i = blockIdx.x; i < r.rows; i += gridDim.x) {
+    T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
+    if (r.mask && !r.mask[i]) {
+      if (threadIdx.x == 0) masked_row(io, i);
+      if (GRAD) zero_row<T, 1024>(dx, r.k, threadIdx.x);
+      continue;
+    }
+    const T* x = (const T*)r.x + i * r.stride;
+    const int64_t c = choice_of(r, i);
+    const bool ok = c >= 0 && c < r.k;
+    const float xc = to_f32(x[ok ? c : 0]);
+    const Part a = stream_part<T, 1024>(x, 0, r.k, slots);
+    const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, threadIdx.x == 0, acc);
+    if (GRAD) stream_grad<T, 1024>(x, dx, 0, r.k, a.m, -e.coef * e.inv, e.coef, c, xc);
+  }
+  if (MODE == POLICY) end_block<1024>(io, blockIdx.x, acc, count, weight, sd);
+}
+
+// Few long rows: `splits` blocks share a row (at most 64), `step` elements each.  First launch: the blocks' (maximum, sum) ...
+template <typename T> __global__ void __launch_bounds__(256) k_split_part(Rows r, int splits, int64_t step, Part* out) {
+  __shared__ Part slots[4];
+  const int64_t i = blockIdx.x / splits, j0 = (blockIdx.x % splits) * step;
+  if (r.mask && !r.mask[i]) return;
+  const Part a = stream_part<T, 256>((const T*)r.x + i * r.stride, j0, min(j0 + step, r.k), slots);
+  if (threadIdx.x == 0) out[blockIdx.x] = a;
+}
+// ... second launch: joined by every block for its own stretch of the gradient; the row's first block writes what belongs to the row.
+template <typename T, int MODE, bool GRAD> __global__ void __launch_bounds__(256) k_split_end(RowIo io, int splits, int64_t step, const Part* parts, int blocks_per_row) {
+  __shared__ double sd[4];
+  double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
+  int64_t count = 0;
+  if (MODE == POLICY) weight = weight_of<256>(io, &count, sd);
+  const Rows& r = io.r;
+  const int64_t i = blockIdx.x / blocks_per_row, j0 = (blockIdx.x % blocks_per_row) * step, j1 = min(j0 + step, r.k);
+  const bool first = j0 == 0 && threadIdx.x == 0;
+  T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
+  if (r.mask && !r.mask[i]) {
+    if (first) masked_row(io, i);
+    if (GRAD) zero_row<T, 256>(dx + j0, j1 - j0, threadIdx.x);
+  } else {
+    const T* x = (const T*)r.x + i * r.stride;
+    const int64_t c = choice_of(r, i);
+    const bool ok = c >= 0 && c < r.k;
+    const float xc = to_f32(x[ok ? c : 0]);
+    const int lane = threadIdx.x & 63;
+    Part a{0.0, -INFINITY};
+    if (lane < splits) a = parts[i * splits + lane];
+    a = join_lanes<64>(a);
+    const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, first, acc);
+    if (GRAD) stream_grad<T, 256>(x, dx, j0, j1, a.m, -e.coef * e.inv, e.coef, c, xc);
+  }
+  if (MODE == POLICY && j0 == 0) {       // (uniform over the block)
+    for (int q = 0; q < 3; ++q)
+      if (threadIdx.x == 0) io.part[i * 3 + q] = acc[q];
   }
 }
 
 // dx = gain * coef (one-hot - p) from the stored statistics (m, 1 / s).  skip_one: dx already holds the result for gain 1.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_rows_grad(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, T* dx) {
+// Rows up to 256 elements: G lanes per row ...
+template <typename T, int G> __global__ void __launch_bounds__(256) k_grad_short(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, T* dx) {
   const float g = gain ? *gain : 1.0f;
   if (skip_one && g == 1.0f) return;
-  for (int64_t i = blockIdx.x; i < r.rows; i += gridDim.x) {
+  const int lane = threadIdx.x & (G - 1), k = (int)r.k;
+  for (int64_t i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; i < r.rows; i += (int64_t)gridDim.x * (256 / G)) {
     const T* x = (const T*)r.x + i * r.stride;
     const float coef = r.mask && !r.mask[i] ? 0.0f : coef_in[i] * g;
     const float2 st = stat[i];
     const int64_t c = choice_of(r, i);
-    for (int64_t j = threadIdx.x; j < r.k; j += kRowThreads)
-      dx[i * r.k + j] = from_f32<T>(coef == 0.0f ? 0.0f : coef * ((j == c ? 1.0f : 0.0f) - exp_of<T>(to_f32(x[j]) - st.x) * st.y));
+    const float scale = -coef * st.y;
+    for (int j = lane; j < k; j += G)
+      dx[i * k + j] = from_f32<T>(coef == 0.0f ? 0.0f : fmaf(exp_of<T>(to_f32(x[j]) - st.x), scale, j == c ? coef : 0.0f));
+  }
+}
+// ... longer rows: blocks of `step` elements, splits of them per row.
+template <typename T> __global__ void __launch_bounds__(256) k_grad_long(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, int splits, int64_t step, T* dx) {
+  const float g = gain ? *gain : 1.0f;
+  if (skip_one && g == 1.0f) return;
+  for (int64_t b = blockIdx.x; b < r.rows * splits; b += gridDim.x) {
+    const int64_t i = b / splits, j0 = (b - i * splits) * step, j1 = min(j0 + step, r.k);
+    const float coef = r.mask && !r.mask[i] ? 0.0f : coef_in[i] * g;
+    if (coef == 0.0f) {
+      zero_row<T, 256>(dx + i * r.k + j0, j1 - j0, threadIdx.x);
+      continue;
+    }
+    const float2 st = stat[i];
+    const T* x = (const T*)r.x + i * r.stride;
+    const int64_t c = choice_of(r, i);
+    stream_grad<T, 256>(x, dx + i * r.k, j0, j1, st.x, -coef * st.y, coef, c, to_f32(x[c >= j0 && c < j1 ? c : j0]));
   }
 }
 
 __global__ void __launch_bounds__(1024) k_count(const uint8_t* mask, int64_t n, int64_t* out) {
   __shared__ double sd[16];
   int64_t c = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) c += mask[i] != 0;
+  for (int64_t i = threadIdx.x; i < n / 16; i += 1024) {
+    Reg<uint8_t> q;
+    q.load(mask + i * 16);
+    c += nonzero_bytes(q);
+  }
+  const int64_t rest = n / 16 * 16 + threadIdx.x;
+  if (threadIdx.x < 16 && rest < n) c += mask[rest] != 0;
   const double t = block_sum<1024>((double)c, sd);     // (counts below 2^53 are exact)
   if (threadIdx.x == 0) *out = (int64_t)t;
 }
 
 // loss, mean kl, clipped share from the blocks' partial sums
-__global__ void __launch_bounds__(256) k_policy_finish(Policy p, int64_t rows, const double* part, int blocks, float* loss, float* kl, float* clip_frac) {
+__global__ void __launch_bounds__(256) k_policy_finish(RowIo io, int64_t blocks) {
   __shared__ double sd[4];
+  int64_t count;
+  const double weight = weight_of<256>(io, &count, sd);
   double v[3] = {0.0, 0.0, 0.0};
-  for (int b = threadIdx.x; b < blocks; b += 256)
-    for (int q = 0; q < 3; ++q) v[q] += part[b * 3 + q];
-  for (int q = 0; q < 3; ++q) v[q] = block_sum<256>(v[q], sd);
-  if (threadIdx.x == 0) {
-    const int64_t n = p.count ? *p.count : rows;
-    const double inv = 1.0 / (double)(n > 0 ? n : 1);
-    *loss = (float)(v[0] * row_weight(p, rows));
-    *kl = (float)(v[1] * inv);
-    *clip_frac = (float)(v[2] * inv);
-  }
+  for (int64_t b = threadIdx.x; b < blocks; b += 256)
+    for (int q = 0; q < 3; ++q) v[q] += io.part[b * 3 + q];
+  end_block<256>(io, 0, v, count, weight, sd);
 }
 
 // ---- preference pairs ------------------------------------------------------------------------------------------------------
@@ -299,20 +697,20 @@ template <typename T> __global__ void __launch_bounds__(256) k_clip_scale(ClipTa
 struct Launches {
   hipStream_t stream;
   hipError_t err = hipSuccess;
-  template <typename... P, size_t... I> void go(void (*k)(P...), int grid, int threads, std::tuple<P...> args, std::index_sequence<I...>) {
+  template <typename... P, size_t... I> void go(void (*k)(P...), dim3 grid, int threads, std::tuple<P...> args, std::index_sequence<I...>) {
     void* ptr[] = {(void*)&std::get<I>(args)...};
-    if (err == hipSuccess) err = hipLaunchKernel((const void*)k, dim3(grid), dim3(threads), ptr, 0, stream);
+    if (err == hipSuccess) err = hipLaunchKernel((const void*)k, grid, dim3(threads), ptr, 0, stream);
   }
-  template <typename... P, typename... A> void operator()(void (*k)(P...), int grid, int threads, A... a) {
+  template <typename... P, typename... A> void operator()(void (*k)(P...), dim3 grid, int threads, A... a) {
     go(k, grid, threads, std::tuple<P...>(a...), std::index_sequence_for<P...>{});
   }
   int result(const char* what) const { return err == hipSuccess ? PS_OK : set_error(PS_E_HIP, "%s: %s", what, hipGetErrorString(err)); }
 };
-int row_grid(int64_t rows) { return (int)(rows < kMaxGrid ? rows : kMaxGrid); }
+int block_grid(int64_t rows) { return (int)(rows < kMaxGrid ? rows : kMaxGrid); }
 
 int check_rows(const ps_decisions* d, const char* what, Rows* r) {
   if (!d) return set_error(PS_E_ARG, "%s: no decisions", what);
-  if (d->rows < 0 || d->choices < 1 || d->choices > (1LL << 31) - 1 || d->rows > (1LL << 40)) return set_error(PS_E_ARG, "%s: rows must be >= 0 and choices in [1, 2^31)", what);
+  if (d->rows < 0 || d->choices < 1 || d->choices > (1LL << 31) - 1 || d->rows > (1LL << 31)) return set_error(PS_E_ARG, "%s: rows must be in [0, 2^31] and choices in [1, 2^31)", what);
   if (d->row_stride < d->choices && d->rows > 1) return set_error(PS_E_ARG, "%s: row_stride < choices", what);
   if (d->dtype != PS_F32 && d->dtype != PS_BF16 && d->dtype != PS_F16) return set_error(PS_E_ARG, "%s: unknown element type", what);
   if (d->choice_bits != 32 && d->choice_bits != 64) return set_error(PS_E_ARG, "%s: choice_bits must be 32 or 64", what);
@@ -325,21 +723,102 @@ template <typename F> int by_type(int dtype, F f) {
   return dtype == PS_F32 ? f((float*)nullptr) : dtype == PS_BF16 ? f((bf16*)nullptr) : f((f16*)nullptr);
 }
 
-struct LossSpace { int64_t* count; double* part; };
-constexpr int64_t kLossSpace = 8 + 24 * (int64_t)kMaxGrid;
+// How rows are laid out over the chip: a rule on their number, length and type.
+struct RowPlan {
+  int kind;             // 0 short, 1 held in registers, 2 long, 3 split
+  int64_t grid;         // blocks
+  int splits;
+  int64_t step;
+};
+constexpr int kShort = 256;            // elements a row of k_rows_short may have (64 lanes x 4)
+RowPlan plan_rows(int64_t rows, int64_t k, int size) {
+  const int64_t bytes = k * size, pieces = k * size / 16;
+  RowPlan p{0, 1, 1, k};
+  auto grid = [&](int64_t per_block, int64_t most) { const int64_t b = (rows + per_block - 1) / per_block; return b < most ? b : most; };
+  if (k <= kShort) {
+    const int g = k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : k <= 64 ? 16 : k <= 128 ? 32 : 64;
+    p.grid = rows * k <= 4096 ? 1 : grid(256 / g, kMaxGrid);
+  } else if (rows <= 128 && bytes >= 32768) {
+    p.kind = 3;
+    const int64_t want = 512 / rows, most = bytes / 8192;
+    p.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
+    if (p.splits > most) p.splits = (int)most;
+    p.step = ((k + p.splits - 1) / p.splits + 63) / 64 * 64;
+    p.splits = (int)((k + p.step - 1) / p.step);
+    p.grid = rows * p.splits;
+  } else if (pieces <= 512) {
+    p.kind = 1;
+    p.grid = (rows + 3) / 4;
+  } else if (pieces <= 16384) {
+    p.kind = 1;
+    p.grid = rows;
+  } else {
+    p.kind = 2;
+    p.grid = grid(1, kMaxGrid);
+  }
+  return p;
+}
+template <typename T, int MODE, bool GRAD> void launch_rows(Launches& run, const RowIo& io, const RowPlan& p, Part* parts) {
+  const int64_t k = io.r.k, pieces = k / Reg<T>::N;
+  const int wide = 1 << 16;
+  const dim3 rows2d(p.grid < wide ? (int)p.grid : wide, (int)((p.grid + wide - 1) / wide));
+  if (p.kind == 0) {
+    if (k <= 4) run(k_rows_short<T, 4, 1, MODE, GRAD>, (int)p.grid, 256, io);
+    else if (k <= 8) run(k_rows_short<T, 8, 1, MODE, GRAD>, (int)p.grid, 256, io);
+    else if (k <= 16) run(k_rows_short<T, 16, 1, MODE, GRAD>, (int)p.grid, 256, io);
+    else if (k <= 64) run(k_rows_short<T, 16, 4, MODE, GRAD>, (int)p.grid, 256, io);
+    else if (k <= 128) run(k_rows_short<T, 32, 4, MODE, GRAD>, (int)p.grid, 256, io);
+    else run(k_rows_short<T, 64, 4, MODE, GRAD>, (int)p.grid, 256, io);
+  } else if (p.kind == 1) {
+    if (pieces <= 128) run(k_rows_held<T, 1, 2, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 512) run(k_rows_held<T, 1, 8, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 1024) run(k_rows_held<T, 4, 4, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 2048) run(k_rows_held<T, 4, 8, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 4096) run(k_rows_held<T, 8, 8, MODE, GRAD>, rows2d, 512, io);
+    else if (pieces <= 8192) run(k_rows_held<T, 16, 8, MODE, GRAD>, rows2d, 1024, io);
+    else run(k_rows_held<T, 16, 16, MODE, GRAD>, rows2d, 1024, io);
+  } else if (p.kind == 2) {
+    run(k_rows_long<T, MODE, GRAD>, (int)p.grid, 1024, io);
+  } else {
+    run(k_split_part<T>, (int)p.grid, 256, io.r, p.splits, p.step, parts);
+    const int per_row = GRAD ? p.splits : 1;
+    run(k_split_end<T, MODE, GRAD>, (int)(io.r.rows * per_row), 256, io, p.splits, p.step, (const Part*)parts, per_row);
+  }
+}
+
+// count | (loss, kl, clipped) per block | partial results of split rows
+int64_t row_space(const ps_decisions* d) {
+  if (!d || d->rows < 1 || d->choices < 1) return 8;
+  const RowPlan p = plan_rows(d->rows, d->choices, d->dtype == PS_F32 ? 4 : 2);
+  return 8 + 24 * (p.kind == 3 ? d->rows : p.grid) + 16 * (p.kind == 3 ? p.grid : 0);
+}
+struct RowSpace {
+  int64_t* count;
+  double* part;
+  Part* parts;
+  RowSpace(void* p, const RowPlan& plan, int64_t rows) : count((int64_t*)p), part((double*)p + 1), parts((Part*)((double*)p + 1 + 3 * (plan.kind == 3 ? rows : plan.grid))) {}
+};
+int check_space(const void* p, int64_t bytes, int64_t need, const char* what) {
+  if (!p || bytes < need || ((uintptr_t)p & 7)) return set_error(PS_E_ARG, "%s: workspace missing, unaligned or smaller than %lld bytes", what, (long long)need);
+  return PS_OK;
+}
 }  // namespace
 
-extern "C" int64_t ps_policy_loss_workspace(const ps_decisions*) { return kLossSpace; }
+extern "C" int64_t ps_choice_workspace(const ps_decisions* d) { return row_space(d); }
 
-extern "C" int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* stream) {
-  Rows r;
-  if (int e = check_rows(d, "ps_choice_logp", &r)) return e;
-  if (!r.rows) return PS_OK;
+extern "C" int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* workspace, int64_t workspace_bytes, void* stream) {
+  RowIo io{};
+  if (int e = check_rows(d, "ps_choice_logp", &io.r)) return e;
+  if (!io.r.rows) return PS_OK;
   if (!logp) return set_error(PS_E_ARG, "ps_choice_logp: NULL logp");
+  if (int e = check_space(workspace, workspace_bytes, row_space(d), "ps_choice_logp")) return e;
   Launches run{(hipStream_t)stream};
+  io.logp = logp;
+  io.stat = (float2*)stat;
   by_type(d->dtype, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
-    run(k_rows<T, LOGP, false>, row_grid(r.rows), kRowThreads, r, Policy{}, logp, (float2*)stat, nullptr, nullptr, nullptr);
+    const RowPlan p = plan_rows(io.r.rows, io.r.k, sizeof(T));
+    launch_rows<T, LOGP, false>(run, io, p, RowSpace(workspace, p, io.r.rows).parts);
     return 0;
   });
   return run.result("ps_choice_logp");
@@ -353,7 +832,17 @@ extern "C" int ps_choice_grad(const ps_decisions* d, const float* coef, const fl
   Launches run{(hipStream_t)stream};
   by_type(d->dtype, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
-    run(k_rows_grad<T>, row_grid(r.rows), kRowThreads, r, coef, (const float2*)stat, gain, skip_if_one, (T*)grad);
+    const float2* st = (const float2*)stat;
+    if (r.k <= kShort) {
+      const int g = r.k <= 4 ? 4 : r.k <= 16 ? 16 : 64;
+      const int64_t b = (r.rows + 256 / g - 1) / (256 / g);
+      run(g == 4 ? k_grad_short<T, 4> : g == 16 ? k_grad_short<T, 16> : k_grad_short<T, 64>, (int)(b < kMaxGrid ? b : kMaxGrid), 256, r, coef, st, gain, skip_if_one, (T*)grad);
+    } else {
+      const int64_t step = 256 * Reg<T>::N * 4;         // 16 KB per block and turn
+      const int splits = (int)((r.k + step - 1) / step);
+      const int64_t b = r.rows < kMaxGrid ? r.rows * splits : kMaxGrid;
+      run(k_grad_long<T>, (int)(b < kMaxGrid ? b : kMaxGrid), 256, r, coef, st, gain, skip_if_one, splits, step, (T*)grad);
+    }
     return 0;
   });
   return run.result("ps_choice_grad");
@@ -361,27 +850,37 @@ extern "C" int ps_choice_grad(const ps_decisions* d, const float* coef, const fl
 
 extern "C" int ps_policy_loss(const ps_decisions* d, const ps_policy_terms* q, float* loss, float* kl, float* clip_frac, float* logp, float* stat,
                               float* coef, void* grad, void* workspace, int64_t workspace_bytes, void* stream) {
-  Rows r;
-  if (int e = check_rows(d, "ps_policy_loss", &r)) return e;
+  RowIo io{};
+  if (int e = check_rows(d, "ps_policy_loss", &io.r)) return e;
+  const Rows& r = io.r;
   if (!q || !loss || !kl || !clip_frac || (r.rows && (!q->old_logp || !q->advantage || !logp))) return set_error(PS_E_ARG, "ps_policy_loss: NULL terms, loss, kl, clip_frac, old_logp, advantage or logp");
   if (!(q->clip_low >= 0.0 && q->clip_low <= 1.0) || !(q->clip_high >= 0.0)) return set_error(PS_E_ARG, "ps_policy_loss: clip_low must be in [0, 1] and clip_high >= 0");
   if (!(q->kl_coef >= 0.0) || std::isinf(q->kl_coef)) return set_error(PS_E_ARG, "ps_policy_loss: kl_coef must be >= 0 and finite");
   if (!std::isfinite(q->scale)) return set_error(PS_E_ARG, "ps_policy_loss: scale must be finite");
   if (q->kl_coef > 0.0 && !q->ref_logp && r.rows) return set_error(PS_E_ARG, "ps_policy_loss: kl_coef without ref_logp");
-  if (!workspace || workspace_bytes < kLossSpace || ((uintptr_t)workspace & 7)) return set_error(PS_E_ARG, "ps_policy_loss: workspace missing, unaligned or smaller than ps_policy_loss_workspace()");
+  if (int e = check_space(workspace, workspace_bytes, row_space(d), "ps_policy_loss")) return e;
   Launches run{(hipStream_t)stream};
-  LossSpace w{(int64_t*)workspace, (double*)workspace + 1};
-  Policy p{q->old_logp, q->advantage, q->ref_logp, 1.0 - q->clip_low, 1.0 + q->clip_high, q->kl_coef, q->scale, r.mask ? w.count : nullptr, q->mean};
-  const int grid = r.rows ? row_grid(r.rows) : 0;
-  if (r.mask) run(k_count, 1, 1024, r.mask, r.rows, w.count);
-  if (grid)
+  const RowPlan p = r.rows ? plan_rows(r.rows, r.k, d->dtype == PS_F32 ? 4 : 2) : RowPlan{0, 0, 1, 0};
+  const RowSpace w(workspace, p, r.rows);
+  const bool counted = r.mask && r.rows > kCountInline;
+  io.p = Policy{q->old_logp, q->advantage, q->ref_logp, 1.0 - q->clip_low, 1.0 + q->clip_high, q->kl_coef, q->scale, counted ? w.count : nullptr, q->mean};
+  io.logp = logp;
+  io.stat = (float2*)stat;
+  io.coef = coef;
+  io.dx = grad;
+  io.part = w.part;
+  io.loss = loss;
+  io.kl = kl;
+  io.clip_frac = clip_frac;
+  if (counted) run(k_count, 1, 1024, r.mask, r.rows, w.count);
+  if (r.rows)
     by_type(d->dtype, [&](auto* t) {
       typedef std::remove_pointer_t<decltype(t)> T;
-      if (grad) run(k_rows<T, POLICY, true>, grid, kRowThreads, r, p, logp, (float2*)stat, coef, (T*)grad, w.part);
-      else run(k_rows<T, POLICY, false>, grid, kRowThreads, r, p, logp, (float2*)stat, coef, (T*)nullptr, w.part);
+      if (grad) launch_rows<T, POLICY, true>(run, io, p, w.parts);
+      else launch_rows<T, POLICY, false>(run, io, p, w.parts);
       return 0;
     });
-  run(k_policy_finish, 1, 256, p, r.rows, w.part, grid, loss, kl, clip_frac);
+  if (p.grid != 1 || p.kind == 3) run(k_policy_finish, 1, 256, io, p.kind == 3 ? r.rows : p.grid);      // (a launch of one block has written the results itself)
   return run.result("ps_policy_loss");
 }
 
@@ -391,9 +890,9 @@ extern "C" int ps_preference_loss(const ps_preference* q, float* loss, float* ma
   if (!q || q->pairs < 1 || q->better_steps < 0 || q->worse_steps < 0) return set_error(PS_E_ARG, "ps_preference_loss: pairs must be >= 1 and steps >= 0");
   if ((q->better_steps && !q->better) || (q->worse_steps && !q->worse) || !loss || !margin || !coef) return set_error(PS_E_ARG, "ps_preference_loss: NULL better, worse, loss, margin or coef");
   if (!std::isfinite(q->beta) || !(q->label_smoothing >= 0.0 && q->label_smoothing <= 1.0) || !std::isfinite(q->scale)) return set_error(PS_E_ARG, "ps_preference_loss: beta and scale must be finite, label_smoothing in [0, 1]");
-  if (!workspace || workspace_bytes < ps_preference_loss_workspace(q->pairs) || ((uintptr_t)workspace & 7)) return set_error(PS_E_ARG, "ps_preference_loss: workspace missing, unaligned or smaller than ps_preference_loss_workspace()");
+  if (int e = check_space(workspace, workspace_bytes, ps_preference_loss_workspace(q->pairs), "ps_preference_loss")) return e;
   Launches run{(hipStream_t)stream};
-  const int grid = row_grid(q->pairs);
+  const int grid = block_grid(q->pairs);
   const double scale = q->scale / (q->mean ? (double)q->pairs : 1.0);
   run(k_pairs, grid, 256, Side{q->better, q->better_ref, q->better_mask, q->better_steps}, Side{q->worse, q->worse_ref, q->worse_mask, q->worse_steps},
                                                  q->pairs, q->beta, q->label_smoothing, scale, margin, coef, (double*)workspace);
@@ -464,7 +963,7 @@ extern "C" int ps_clip_grads(int32_t n, void* const* ptr, const int64_t* numel, 
   if (!norm) return set_error(PS_E_ARG, "ps_clip_grads: NULL norm");
   const int64_t need = ps_clip_grads_workspace(n, numel);
   if (need > (1LL << 31)) return set_error(PS_E_ARG, "ps_clip_grads: more than 2^43 elements");
-  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 7)) return set_error(PS_E_ARG, "ps_clip_grads: workspace missing, unaligned or smaller than ps_clip_grads_workspace()");
+  if (int e = check_space(workspace, workspace_bytes, need, "ps_clip_grads")) return e;
   Launches run{(hipStream_t)stream};
   float* coef = (float*)workspace;
   double* part = (double*)workspace + 1;

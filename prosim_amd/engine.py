@@ -137,16 +137,16 @@ def load_library():
     lib.ps_test_get_edges.restype = C.c_int64
     lib.ps_test_stream.argtypes = [vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, fp]
     dec = C.POINTER(PsDecisions)
-    lib.ps_choice_logp.argtypes = [dec, vp, vp, vp]
+    lib.ps_choice_logp.argtypes = [dec, vp, vp, vp, C.c_int64, vp]
     lib.ps_choice_grad.argtypes = [dec, vp, vp, vp, C.c_int32, vp, vp]
     lib.ps_policy_loss.argtypes = [dec, C.POINTER(PsPolicyTerms), vp, vp, vp, vp, vp, vp, vp, vp, C.c_int64, vp]
     lib.ps_preference_loss.argtypes = [C.POINTER(PsPreference), vp, vp, vp, vp, C.c_int64, vp]
     lib.ps_preference_grad.argtypes = [C.POINTER(PsPreference), vp, vp, vp, vp, vp]
     lib.ps_clip_grads.argtypes = [C.c_int32, vp, vp, vp, C.c_double, C.c_double, vp, vp, C.c_int64, vp]
-    lib.ps_policy_loss_workspace.argtypes = [dec]
+    lib.ps_choice_workspace.argtypes = [dec]
     lib.ps_preference_loss_workspace.argtypes = [C.c_int64]
     lib.ps_clip_grads_workspace.argtypes = [C.c_int32, vp]
-    for name in ("ps_policy_loss_workspace", "ps_preference_loss_workspace", "ps_clip_grads_workspace"):
+    for name in ("ps_choice_workspace", "ps_preference_loss_workspace", "ps_clip_grads_workspace"):
         getattr(lib, name).restype = C.c_int64
     _lib = lib
     return lib
@@ -155,7 +155,7 @@ def load_library():
 EXPORTS = ["ps_create", "ps_destroy", "ps_last_error", "ps_set_scene", "ps_set_prompt", "ps_policy_forward", "ps_set_conditions", "ps_set_drag_points", "ps_set_pair_conditions", "ps_set_future_obs", "ps_set_future_log", "ps_set_mode_choice", "ps_set_action_noise", "ps_set_replicas", "ps_num_replicas", "ps_world_trajs", "ps_num_policy_agents", "ps_policy_flags",
            "ps_encode_scene", "ps_generate_policy", "ps_reset_rollout", "ps_policy_step", "ps_rollout", "ps_sync", "ps_stream", "ps_set_chain_rows", "ps_set_chain_impl", "ps_set_row_impl", "ps_set_search_impl", "ps_graph_nodes", "ps_enable_policy_events", "ps_policy_event_times", "ps_update_obs", "ps_set_map_tokens", "ps_declare_agent_rows",
            "ps_set_state", "ps_get", "ps_get_async", "ps_graph_stats", "ps_rollout_metric", "ps_pair_metric", "ps_num_agents", "ps_num_map_tokens", "ps_time_rollout", "ps_time_policy_kernel",
-           "ps_choice_logp", "ps_choice_grad", "ps_policy_loss", "ps_policy_loss_workspace", "ps_preference_loss", "ps_preference_loss_workspace", "ps_preference_grad", "ps_clip_grads", "ps_clip_grads_workspace",
+           "ps_choice_logp", "ps_choice_grad", "ps_policy_loss", "ps_choice_workspace", "ps_preference_loss", "ps_preference_loss_workspace", "ps_preference_grad", "ps_clip_grads", "ps_clip_grads_workspace",
            "ps_test_pointnet", "ps_test_pointnet_mt", "ps_test_fourier", "ps_test_wrap", "ps_test_attn", "ps_test_get_edges", "ps_test_stream"]
 
 

@@ -152,13 +152,21 @@ def _reduction(name: str) -> int:
 
 # ---- log-probability of a choice -------------------------------------------------------------------------------------
 
+def _logp_forward(logits, choice, mask, stat):
+    lib, dev = load_library(), logits.device
+    rows = _rows(logits)
+    d = _decisions(rows, choice, mask)
+    logp = torch.empty(choice.shape, dtype=torch.float32, device=dev)
+    space = torch.empty(lib.ps_choice_workspace(d), dtype=torch.uint8, device=dev)
+    _call(dev, lib.ps_choice_logp, d, logp.data_ptr(), _ptr(stat), space.data_ptr(), space.numel())
+    return logp
+
+
 class _ChoiceLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, choice, mask):
-        rows = _rows(logits)
-        logp = torch.empty(choice.shape, dtype=torch.float32, device=logits.device)
         stat = torch.empty((choice.numel(), 2), dtype=torch.float32, device=logits.device)
-        _call(logits.device, load_library().ps_choice_logp, _decisions(rows, choice, mask), logp.data_ptr(), stat.data_ptr())
+        logp = _logp_forward(logits, choice, mask, stat)
         ctx.save_for_backward(logits, choice, mask, stat)
         return logp
 
@@ -188,10 +196,7 @@ def choice_logp(logits: torch.Tensor, choice: torch.Tensor, *, mask: Optional[to
     _, choice, mask = _check_decisions(logits, choice, mask)
     if logits.requires_grad and torch.is_grad_enabled():
         return _ChoiceLogp.apply(logits, choice, mask)
-    rows = _rows(logits)
-    logp = torch.empty(choice.shape, dtype=torch.float32, device=logits.device)
-    _call(logits.device, load_library().ps_choice_logp, _decisions(rows, choice, mask), logp.data_ptr(), None)
-    return logp
+    return _logp_forward(logits, choice, mask, None)
 
 
 # ---- clipped policy loss ---------------------------------------------------------------------------------------------
@@ -202,7 +207,7 @@ def _policy_forward(logits, choice, mask, terms: PsPolicyTerms, grad, stat, coef
     logp = torch.empty(choice.shape, dtype=torch.float32, device=dev)
     rows = _rows(logits)
     d = _decisions(rows, choice, mask)
-    space = torch.empty(lib.ps_policy_loss_workspace(d), dtype=torch.uint8, device=dev)
+    space = torch.empty(lib.ps_choice_workspace(d), dtype=torch.uint8, device=dev)
     _call(dev, lib.ps_policy_loss, d, terms, loss.data_ptr(), kl.data_ptr(), frac.data_ptr(), logp.data_ptr(), _ptr(stat), _ptr(coef), _ptr(grad),
           space.data_ptr(), space.numel())
     return loss, logp, kl, frac

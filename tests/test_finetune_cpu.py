@@ -29,7 +29,7 @@ def _d(**kw):
                                  dict(logits=None), dict(choice=None)])
 def test_c_entries_refuse_bad_decisions(lib, bad):
     d = _d(**bad)
-    assert lib.ps_choice_logp(d, FAKE, None, None) == -1
+    assert lib.ps_choice_logp(d, FAKE, None, FAKE, 1 << 20, None) == -1
     assert lib.ps_last_error().startswith(b"ps_choice_logp: ")
     assert lib.ps_choice_grad(d, FAKE, FAKE, None, 0, FAKE, None) == -1
     t = PsPolicyTerms(FAKE, FAKE, None, 0.2, 0.2, 0.0, 1.0, 1)
@@ -38,11 +38,11 @@ def test_c_entries_refuse_bad_decisions(lib, bad):
 
 
 def test_c_entries_refuse_missing_buffers(lib):
-    assert lib.ps_choice_logp(None, FAKE, None, None) == -1
-    assert lib.ps_choice_logp(_d(), None, None, None) == -1
+    assert lib.ps_choice_logp(None, FAKE, None, FAKE, 1 << 20, None) == -1
+    assert lib.ps_choice_logp(_d(), None, None, FAKE, 1 << 20, None) == -1
     for args in ((None, FAKE, FAKE), (FAKE, None, FAKE), (FAKE, FAKE, None)):
         assert lib.ps_choice_grad(_d(), args[0], args[1], None, 0, args[2], None) == -1
-    assert lib.ps_choice_logp(_d(rows=0, logits=None, choice=None), None, None, None) == 0     # (no rows: nothing to do)
+    assert lib.ps_choice_logp(_d(rows=0, logits=None, choice=None), None, None, None, 0, None) == 0     # (no rows: nothing to do)
 
 
 @pytest.mark.parametrize("bad", [dict(old_logp=None), dict(advantage=None), dict(clip_low=-0.1), dict(clip_low=1.5), dict(clip_low=float("nan")), dict(clip_high=-1.0),
@@ -58,10 +58,11 @@ def test_policy_loss_terms(lib, bad):
 
 def test_workspaces_are_checked(lib):
     t = PsPolicyTerms(FAKE, FAKE, None, 0.2, 0.2, 0.0, 1.0, 1)
-    need = lib.ps_policy_loss_workspace(_d())
+    need = lib.ps_choice_workspace(_d())
     assert need > 0
     for ws, size in ((None, need), (FAKE, need - 1), (FAKE + 4, need)):
         assert lib.ps_policy_loss(_d(), t, FAKE, FAKE, FAKE, FAKE, None, None, None, ws, size, None) == -1
+        assert lib.ps_choice_logp(_d(), FAKE, None, ws, size, None) == -1
     q = PsPreference(FAKE, None, FAKE, None, None, None, 2, 3, 3, 0.1, 0.0, 1.0, 1)
     need = lib.ps_preference_loss_workspace(2)
     for ws, size in ((None, need), (FAKE, need - 1), (FAKE + 4, need)):
