@@ -5,7 +5,6 @@ import numpy as np
 import pytest
 import torch
 
-from prosim_amd import finetune
 from prosim_amd.engine import PsDecisions, PsPolicyTerms, PsPreference, load_library
 
 
@@ -101,7 +100,8 @@ def test_clip_tables_are_checked(lib):
     assert b"ps_clip_grads" in lib.ps_last_error()
 
 
-def test_there_is_no_cpu_fallback():
+def test_there_is_no_cpu_fallback(lib):
+    from prosim_amd import finetune
     x, c = torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64)
     with pytest.raises(ValueError):
         finetune.choice_logp(x, c)
@@ -117,23 +117,18 @@ def test_there_is_no_cpu_fallback():
         finetune.clip_grads_([None], 1.0)
 
 
-def test_dense_and_row_strides():
+def test_dense_and_row_strides(lib):
     """The layouts the operators take without a copy."""
+    from prosim_amd import _finetune
+    dense, stride = _finetune.dense, _finetune.row_stride
     t = torch.zeros(4, 5, 6)
-    assert finetune._dense(t) and finetune._dense(t.permute(2, 0, 1)) and finetune._dense(t[:1]) and finetune._dense(torch.zeros(()))
-    assert not finetune._dense(t[:, :4]) and not finetune._dense(t[..., ::2]) and not finetune._dense(torch.zeros(1).expand(3))
+    assert dense(t) and dense(t.permute(2, 0, 1)) and dense(t[:1]) and dense(torch.zeros(()))
+    assert not dense(t[:, :4]) and not dense(t[..., ::2]) and not dense(torch.zeros(1).expand(3))
     pad = torch.zeros(7, 4, 16)
-    v = pad[..., :9]
-    assert finetune._rows(v).data_ptr() == v.data_ptr() and finetune._row_stride(v) == 16
-    v = pad[:, 1, :9]
-    assert finetune._rows(v) is v and finetune._row_stride(v) == 64
-    v = pad[:, :3, :9]                        # two strides: copied
-    assert finetune._rows(v).is_contiguous()
-    v = pad[:, :1, :9]                        # the middle dimension has one entry: one stride
-    assert finetune._rows(v) is v and finetune._row_stride(v) == 64
-    v = torch.zeros(16).expand(5, 16)         # rows on top of each other: copied
-    assert finetune._rows(v).is_contiguous()
-    v = pad.transpose(1, 2)
-    assert finetune._rows(v).is_contiguous()
-    v = torch.zeros(9)
-    assert finetune._rows(v) is v and finetune._row_stride(v) == 9
+    assert stride(pad) == 16 and stride(pad[..., :9]) == 16
+    assert stride(pad[:, 1, :9]) == 64
+    assert stride(pad[:, :3, :9]) == -1                  # two strides: copied
+    assert stride(pad[:, :1, :9]) == 64                  # the middle dimension has one entry: one stride
+    assert stride(torch.zeros(16).expand(5, 16)) == -1   # rows on top of each other: copied
+    assert stride(pad.transpose(1, 2)) == -1 and stride(pad[..., ::2]) == -1
+    assert stride(pad[..., :1]) == 16 and stride(torch.zeros(9)) == 9

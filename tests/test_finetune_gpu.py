@@ -457,6 +457,10 @@ def test_refusals(ft):
             bad()
     with pytest.raises(TypeError):
         ft.clip_grads_([x.double()], 1.0)
+    leaf = x.clone().requires_grad_(True)            # a gradient of a gradient
+    g, = torch.autograd.grad((ft.choice_logp(leaf, c) ** 2).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
     with pytest.raises(RuntimeError):                # changed between the passes: autograd's own check
         leaf = (x + 1).requires_grad_(True)
         y = ft.choice_logp(leaf * 1.0, c)
