@@ -392,7 +392,7 @@ int ps_preference_grad(const ps_preference* q, const float* coef, const float* g
 /* Gradient clipping by the global norm, in place: norm [1] = sqrt(sum of squares over all n tensors), and every element is multiplied by
  * min(1, max_norm / (norm + eps)) (not touched when that is 1; max_norm = inf only measures; a NaN norm makes NaN gradients).  HOST tables:
  * ptr [n] device pointers to dense tensors that do not overlap, numel [n], dtype [n] (PS_F32 ...); read before the call returns. */
-int64_t ps_clip_grads_workspace(int32_t n, const int64_t* numel);
+int64_t ps_clip_grads_workspace(int32_t n, const int64_t* numel, const int32_t* dtype);
 int ps_clip_grads(int32_t n, void* const* ptr, const int64_t* numel, const int32_t* dtype, double max_norm, double eps, float* norm,
                   void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -642,34 +642,53 @@ __global__ void __launch_bounds__(256) k_pairs_grad(const float* coef, const flo
 }
 
 // ---- gradient lists --------------------------------------------------------------------------------------------------------
-constexpr int kClipSlots = 240;          // tensors of a launch: the table travels in the kernel's arguments (under 4 KB), no copy to wait for
-constexpr int64_t kClipChunk = 32768;    // elements of a block
+constexpr int kClipSlots = 240;          // ranges of a launch: the table travels in the kernel's arguments (under 4 KB), no copy to wait for
+constexpr int kClipPieces = 8;           // 16-byte pieces of a thread, all in flight at once: 32 KB per block
+template <typename T> constexpr int64_t clip_chunk() { return 256 * kClipPieces * Reg<T>::N; }      // elements of a block
 struct ClipTable {
   void* ptr[kClipSlots];
   uint32_t numel[kClipSlots];
-  int32_t first[kClipSlots];             // first block of the tensor
-  int n, block0;                         // block0: index of the launch's first block among the partial sums
+  int32_t first[kClipSlots];             // first block of the range
+  int n, blocks, block0;                 // block0: index of the launch's first block among the partial sums
 };
-__device__ __forceinline__ int clip_slot(const ClipTable& t, int b) {
+// the elements [a, e) of range s that block b has
+template <typename T> __device__ __forceinline__ T* clip_part(const ClipTable& t, int b, int* len) {
   int lo = 0, hi = t.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (t.first[mid] <= b) lo = mid; else hi = mid - 1;
   }
-  return lo;
+  const int64_t a = (int64_t)(b - t.first[lo]) * clip_chunk<T>();
+  *len = (int)min(clip_chunk<T>(), (int64_t)t.numel[lo] - a);
+  return (T*)t.ptr[lo] + a;
 }
+// Sum of squares of a block's elements, in 64 bits from the square on (a 32-bit square overflows from 1.8e19 and vanishes below 3.7e-23).
 template <typename T> __global__ void __launch_bounds__(256) k_clip_norm(ClipTable t, double* part) {
+  constexpr int V = Reg<T>::N;
   __shared__ double sd[4];
-  const int s = clip_slot(t, blockIdx.x);
-  const int64_t a = (int64_t)(blockIdx.x - t.first[s]) * kClipChunk, e = min(a + kClipChunk, (int64_t)t.numel[s]);
-  const T* g = (const T*)t.ptr[s];
-  double v = 0.0;
-  for (int64_t j = a + threadIdx.x; j < e; j += 256) {
-    const double d = (double)to_f32(g[j]);
-    v += d * d;
+  int len;
+  const T* g = clip_part<T>(t, blockIdx.x, &len);
+  const int n = len / V;
+  Reg<T> v[kClipPieces];
+#pragma unroll
+  for (int q = 0; q < kClipPieces; ++q) {
+    v[q].w[0] = v[q].w[1] = v[q].w[2] = v[q].w[3] = 0;
+    if (q * 256 + (int)threadIdx.x < n) v[q].load(g + q * (256 * V) + threadIdx.x * V);
   }
-  v = block_sum<256>(v, sd);
-  if (threadIdx.x == 0) part[t.block0 + blockIdx.x] = v;
+  double a = 0.0;
+  if (n * V + (int)threadIdx.x < len) {
+    const double d = (double)to_f32(g[n * V + threadIdx.x]);
+    a = d * d;
+  }
+#pragma unroll
+  for (int q = 0; q < kClipPieces; ++q) {
+    float f[V];
+    v[q].get(f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) a = fma((double)f[j], (double)f[j], a);
+  }
+  a = block_sum<256>(a, sd);
+  if (threadIdx.x == 0) part[t.block0 + blockIdx.x] = a;
 }
 __global__ void __launch_bounds__(1024) k_clip_finish(const double* part, int64_t blocks, double max_norm, double eps, float* norm, float* coef) {
   __shared__ double sd[16];
@@ -682,13 +701,32 @@ __global__ void __launch_bounds__(1024) k_clip_finish(const double* part, int64_
     *coef = c >= 1.0 ? 1.0f : (float)c;       // (a NaN norm makes NaN gradients)
   }
 }
+// The last block first: what the norm's pass read last is still in the 256 MB cache.
 template <typename T> __global__ void __launch_bounds__(256) k_clip_scale(ClipTable t, const float* coef) {
+  constexpr int V = Reg<T>::N;
   const float c = *coef;
   if (c == 1.0f) return;
-  const int s = clip_slot(t, blockIdx.x);
-  const int64_t a = (int64_t)(blockIdx.x - t.first[s]) * kClipChunk, e = min(a + kClipChunk, (int64_t)t.numel[s]);
-  T* g = (T*)t.ptr[s];
-  for (int64_t j = a + threadIdx.x; j < e; j += 256) g[j] = from_f32<T>(to_f32(g[j]) * c);
+  int len;
+  T* g = clip_part<T>(t, t.blocks - 1 - blockIdx.x, &len);
+  const int n = len / V;
+  Reg<T> v[kClipPieces];
+#pragma unroll
+  for (int q = 0; q < kClipPieces; ++q)
+    if (q * 256 + (int)threadIdx.x < n) v[q].load(g + q * (256 * V) + threadIdx.x * V);
+  if (n * V + (int)threadIdx.x < len) {
+    T* e = g + n * V + threadIdx.x;
+    *e = from_f32<T>(to_f32(*e) * c);
+  }
+#pragma unroll
+  for (int q = 0; q < kClipPieces; ++q)
+    if (q * 256 + (int)threadIdx.x < n) {
+      float f[V];
+      v[q].get(f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] *= c;
+      v[q].set(f);
+      v[q].store(g + q * (256 * V) + threadIdx.x * V);
+    }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
@@ -911,7 +949,10 @@ extern "C" int ps_preference_grad(const ps_preference* q, const float* coef, con
 }
 
 namespace {
-int64_t clip_blocks(int64_t n) { return (n + kClipChunk - 1) / kClipChunk; }
+int64_t clip_blocks(int64_t n, int dtype) {
+  const int64_t chunk = dtype == PS_F32 ? clip_chunk<float>() : clip_chunk<bf16>();
+  return (n + chunk - 1) / chunk;
+}
 constexpr int64_t kClipPiece = 1LL << 31;     // elements of a table entry (a longer tensor takes several)
 int check_clip(const char* what, int32_t n, void* const* ptr, const int64_t* numel, const int32_t* dtype) {
   if (n < 0 || (n && (!ptr || !numel || !dtype))) return set_error(PS_E_ARG, "%s: NULL table", what);
@@ -920,8 +961,8 @@ int check_clip(const char* what, int32_t n, void* const* ptr, const int64_t* num
       return set_error(PS_E_ARG, "%s: tensor %d has a negative size, a NULL or unaligned pointer or an unknown element type", what, (int)i);
   return PS_OK;
 }
-// fill one table after the other, each of one element type, and launch it
-template <typename F> void clip_tables(int32_t n, void* const* ptr, const int64_t* numel, const int32_t* dtype, F launch) {
+// fill one table after the other, each of one element type, and launch it; returns the blocks of all launches
+template <typename F> int64_t clip_tables(int32_t n, void* const* ptr, const int64_t* numel, const int32_t* dtype, F launch) {
   ClipTable t;
   int64_t block0 = 0;
   for (int ty : {PS_F32, PS_BF16, PS_F16}) {
@@ -933,6 +974,7 @@ template <typename F> void clip_tables(int32_t n, void* const* ptr, const int64_
       for (int64_t a = 0; i == n || a < numel[i]; a += kClipPiece) {
         if (t.n && (i == n || t.n == kClipSlots || blocks > (1 << 21))) {
           t.block0 = (int)block0;
+          t.blocks = blocks;
           launch(t, blocks, ty);
           block0 += blocks;
           blocks = 0;
@@ -943,16 +985,17 @@ template <typename F> void clip_tables(int32_t n, void* const* ptr, const int64_
         t.ptr[t.n] = (char*)ptr[i] + a * size;
         t.numel[t.n] = (uint32_t)len;
         t.first[t.n++] = blocks;
-        blocks += (int)clip_blocks(len);
+        blocks += (int)clip_blocks(len, ty);
       }
     }
   }
+  return block0;
 }
 }  // namespace
 
-extern "C" int64_t ps_clip_grads_workspace(int32_t n, const int64_t* numel) {
+extern "C" int64_t ps_clip_grads_workspace(int32_t n, const int64_t* numel, const int32_t* dtype) {
   int64_t b = 0;
-  for (int32_t i = 0; i < n; ++i) b += clip_blocks(numel[i] > 0 ? numel[i] : 0);
+  for (int32_t i = 0; i < n; ++i) b += clip_blocks(numel[i] > 0 ? numel[i] : 0, dtype[i]);
   return 8 * (b + 1);
 }
 
@@ -961,16 +1004,16 @@ extern "C" int ps_clip_grads(int32_t n, void* const* ptr, const int64_t* numel, 
   if (int e = check_clip("ps_clip_grads", n, ptr, numel, dtype)) return e;
   if (!(max_norm >= 0.0) || !(eps >= 0.0) || std::isinf(eps)) return set_error(PS_E_ARG, "ps_clip_grads: max_norm must be >= 0, eps >= 0 and finite");
   if (!norm) return set_error(PS_E_ARG, "ps_clip_grads: NULL norm");
-  const int64_t need = ps_clip_grads_workspace(n, numel);
-  if (need > (1LL << 31)) return set_error(PS_E_ARG, "ps_clip_grads: more than 2^43 elements");
+  const int64_t need = ps_clip_grads_workspace(n, numel, dtype);
+  if (need / 8 > (1LL << 30)) return set_error(PS_E_ARG, "ps_clip_grads: more than 2^43 elements");
   if (int e = check_space(workspace, workspace_bytes, need, "ps_clip_grads")) return e;
   Launches run{(hipStream_t)stream};
   float* coef = (float*)workspace;
   double* part = (double*)workspace + 1;
-  clip_tables(n, ptr, numel, dtype, [&](const ClipTable& t, int blocks, int ty) {
+  const int64_t blocks = clip_tables(n, ptr, numel, dtype, [&](const ClipTable& t, int blocks, int ty) {
     by_type(ty, [&](auto* p) { run(k_clip_norm<std::remove_pointer_t<decltype(p)>>, blocks, 256, t, part); return 0; });
   });
-  run(k_clip_finish, 1, 1024, part, need / 8 - 1, max_norm, eps, norm, coef);
+  run(k_clip_finish, 1, 1024, part, blocks, max_norm, eps, norm, coef);
   clip_tables(n, ptr, numel, dtype, [&](const ClipTable& t, int blocks, int ty) {
     by_type(ty, [&](auto* p) { run(k_clip_scale<std::remove_pointer_t<decltype(p)>>, blocks, 256, t, coef); return 0; });
   });

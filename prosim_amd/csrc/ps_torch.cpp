@@ -197,6 +197,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     ctx->saved_data["ready"] = grad;
     ctx->save_for_backward({logits, rest.choice, rest.mask, space.all});
     ctx->mark_non_differentiable({out[1], out[2], out[3]});
+    ctx->set_materialize_grads(false);        // (no zeros for the three numbers that carry no gradient)
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -245,6 +246,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     ctx->saved_data["better"] = better.sizes();
     ctx->saved_data["worse"] = worse.sizes();
     ctx->mark_non_differentiable({margin});
+    ctx->set_materialize_grads(false);
     return {loss, margin};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -296,28 +298,43 @@ Tensor clip_grads(const py::list& list, double max_norm, double eps) {
     ts.push_back(THPVariable_Unpack(h.ptr()));
   }
   TORCH_CHECK_VALUE(!ts.empty(), "clip_grads_: no gradients");
-  const size_t n = ts.size();
-  std::vector<void*> at(n);
-  std::vector<int64_t> numel(n);
-  std::vector<int32_t> dtype(n);
-  std::vector<std::pair<uintptr_t, uintptr_t>> used;
-  used.reserve(n);
-  for (size_t i = 0; i < n; ++i) {
-    const Tensor& t = ts[i];
+  // Ranges of memory, by address: that finds tensors on top of each other, and makes one range of neighbours -- data-parallel training keeps its
+  // gradients as views of a few flat buffers, hundreds of tensors that are then a handful of ranges.
+  struct Range { uintptr_t begin, end; int32_t dtype; };
+  std::vector<Range> used;
+  used.reserve(ts.size());
+  bool sorted = true;
+  for (const Tensor& t : ts) {
     check_gpu(t, "grads", ts[0]);
-    dtype[i] = dtype_of(t);
-    TORCH_CHECK_TYPE(dtype[i] >= 0, "grads: expected float32, bfloat16 or float16, got ", type_name(t));
+    const int dtype = dtype_of(t);
+    TORCH_CHECK_TYPE(dtype >= 0, "grads: expected float32, bfloat16 or float16, got ", type_name(t));
     TORCH_CHECK_VALUE(!t.requires_grad(), "grads: a tensor requires a gradient itself (parameters instead of their gradients?)");
     TORCH_CHECK_VALUE(dense(t), "grads: a tensor of shape ", t.sizes(), " and strides ", t.strides(), " is not dense");
-    numel[i] = t.numel();
-    at[i] = numel[i] ? t.data_ptr() : nullptr;
-    if (numel[i]) used.emplace_back((uintptr_t)at[i], (uintptr_t)at[i] + numel[i] * t.element_size());
+    if (!t.numel()) continue;
+    const uintptr_t begin = (uintptr_t)t.data_ptr();
+    sorted = sorted && (used.empty() || used.back().begin <= begin);
+    used.push_back(Range{begin, begin + t.numel() * t.element_size(), dtype});
   }
-  if (!std::is_sorted(used.begin(), used.end())) std::sort(used.begin(), used.end());
-  for (size_t i = 1; i < used.size(); ++i) TORCH_CHECK_VALUE(used[i - 1].second <= used[i].first, "grads: two tensors share memory");
+  if (!sorted) std::sort(used.begin(), used.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  std::vector<void*> at;
+  std::vector<int64_t> numel;
+  std::vector<int32_t> dtypes;
+  for (size_t i = 0; i < used.size(); ++i) {
+    const Range& r = used[i];
+    const int64_t n = (r.end - r.begin) / (r.dtype == PS_F32 ? 4 : 2);
+    TORCH_CHECK_VALUE(!i || used[i - 1].end <= r.begin, "grads: two tensors share memory");
+    if (i && used[i - 1].end == r.begin && dtypes.back() == r.dtype) {
+      numel.back() += n;
+    } else {
+      at.push_back((void*)r.begin);
+      numel.push_back(n);
+      dtypes.push_back(r.dtype);
+    }
+  }
+  const int32_t n = (int32_t)at.size();
   const c10::DeviceGuard guard(ts[0].device());
-  const Tensor norm = empty({}, ts[0]), space = empty({ps_clip_grads_workspace((int32_t)n, numel.data())}, ts[0], at::kByte);
-  check(ps_clip_grads((int32_t)n, at.data(), numel.data(), dtype.data(), max_norm, eps, ptr<float>(norm), space.data_ptr(), space.numel(), stream_of(ts[0])));
+  const Tensor norm = empty({}, ts[0]), space = empty({ps_clip_grads_workspace(n, numel.data(), dtypes.data())}, ts[0], at::kByte);
+  check(ps_clip_grads(n, at.data(), numel.data(), dtypes.data(), max_norm, eps, ptr<float>(norm), space.data_ptr(), space.numel(), stream_of(ts[0])));
   for (const Tensor& t : ts)
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   return norm;

@@ -145,7 +145,7 @@ def load_library():
     lib.ps_clip_grads.argtypes = [C.c_int32, vp, vp, vp, C.c_double, C.c_double, vp, vp, C.c_int64, vp]
     lib.ps_choice_workspace.argtypes = [dec]
     lib.ps_preference_loss_workspace.argtypes = [C.c_int64]
-    lib.ps_clip_grads_workspace.argtypes = [C.c_int32, vp]
+    lib.ps_clip_grads_workspace.argtypes = [C.c_int32, vp, vp]
     for name in ("ps_choice_workspace", "ps_preference_loss_workspace", "ps_clip_grads_workspace"):
         getattr(lib, name).restype = C.c_int64
     _lib = lib

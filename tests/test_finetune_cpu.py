@@ -94,8 +94,8 @@ def test_clip_tables_are_checked(lib):
     assert call([FAKE], [4], [0], norm=None) == -1
     assert call([FAKE], [4], [0], ws=None) == -1
     assert call([FAKE], [4], [0], size=8) == -1
-    n = np.array([1, 0, 1 << 33], np.int64)
-    assert lib.ps_clip_grads_workspace(3, n.ctypes.data) > 8
+    n, t = np.array([1, 0, 1 << 33], np.int64), np.array([0, 1, 2], np.int32)
+    assert lib.ps_clip_grads_workspace(3, n.ctypes.data, t.ctypes.data) > 8
     assert lib.ps_clip_grads(1, None, None, None, 1.0, 1e-6, FAKE, FAKE, 1 << 20, None) == -1
     assert b"ps_clip_grads" in lib.ps_last_error()
 
