@@ -61,6 +61,19 @@ template <int THREADS> __device__ __forceinline__ float block_max(float v, float
   return t;
 }
 
+// sum of n numbers by one block, eight loads in flight per thread
+template <int THREADS> __device__ __forceinline__ double long_sum(const double* part, int64_t n, int64_t stride) {
+  double v = 0.0;
+  for (int64_t b = threadIdx.x; b < n; b += 8 * THREADS) {
+    double u[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) u[q] = b + q * THREADS < n ? part[(b + q * THREADS) * stride] : 0.0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += u[q];
+  }
+  return v;
+}
+
 // ---- rows of decisions -----------------------------------------------------------------------------------------------------
 struct Rows {
   const void* x;          // [rows][stride], the first k of a row are its logits
@@ -595,50 +608,100 @@ __global__ void __launch_bounds__(256) k_policy_finish(RowIo io, int64_t blocks)
   __shared__ double sd[4];
   int64_t count;
   const double weight = weight_of<256>(io, &count, sd);
-  double v[3] = {0.0, 0.0, 0.0};
-  for (int64_t b = threadIdx.x; b < blocks; b += 256)
-    for (int q = 0; q < 3; ++q) v[q] += io.part[b * 3 + q];
+  double v[3];
+  for (int q = 0; q < 3; ++q) v[q] = long_sum<256>(io.part + q, blocks, 3);
   end_block<256>(io, 0, v, count, weight, sd);
 }
 
 // ---- preference pairs ------------------------------------------------------------------------------------------------------
 struct Side { const float *logp, *ref; const uint8_t* mask; int64_t steps; };
-__device__ __forceinline__ double side_sum(const Side& s, int64_t p) {
+struct __attribute__((packed)) Bytes4 { uint32_t w; };
+// sum of the log ratios of pair p's valid steps by TPP threads, four steps a piece; masked steps are read with their piece and dropped by selection
+template <int TPP> __device__ __forceinline__ double side_sum(const Side& s, int64_t p, int t) {
+  const float *a = s.logp + p * s.steps, *r = s.ref ? s.ref + p * s.steps : nullptr;
+  const uint8_t* m = s.mask ? s.mask + p * s.steps : nullptr;
+  const int64_t n = s.steps / 4;
   double v = 0.0;
-  for (int64_t t = threadIdx.x; t < s.steps; t += 256) {
-    const int64_t j = p * s.steps + t;
-    if (s.mask && !s.mask[j]) continue;
-    v += (double)s.logp[j] - (s.ref ? (double)s.ref[j] : 0.0);
-  }
-  return v;
-}
-__global__ void __launch_bounds__(256) k_pairs(Side w, Side l, int64_t pairs, double beta, double eps, double scale, float* margin, float* coef, double* part) {
-  __shared__ double sd[4];
-  double loss = 0.0;
-  for (int64_t p = blockIdx.x; p < pairs; p += gridDim.x) {
-    const double h = block_sum<256>(side_sum(w, p) - side_sum(l, p), sd);
-    if (threadIdx.x == 0) {
-      const double z = beta * h, e = exp(-fabs(z)), lp = log1p(e);
-      const double neg = (z < 0.0 ? -z : 0.0) + lp, pos = (z > 0.0 ? z : 0.0) + lp;      // -ln sigmoid(z), -ln sigmoid(-z)
-      const double down = z >= 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e), up = z >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);   // sigmoid(-z), sigmoid(z)
-      margin[p] = (float)z;
-      coef[p] = (float)(scale * beta * (eps * up - (1.0 - eps) * down));
-      loss += z != z ? z : (1.0 - eps) * neg + eps * pos;
+#pragma unroll 4
+  for (int64_t q = t; q < n; q += TPP) {
+    Reg<float> x, y;
+    y.w[0] = y.w[1] = y.w[2] = y.w[3] = 0;
+    uint32_t keep = 0xffffffffu;
+    x.load(a + q * 4);
+    if (r) y.load(r + q * 4);
+    if (m) keep = ((const Bytes4*)(m + q * 4))->w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double d = (double)__uint_as_float(x.w[j]) - (double)__uint_as_float(y.w[j]);
+      v += keep >> 8 * j & 255u ? d : 0.0;
     }
   }
-  if (threadIdx.x == 0) part[blockIdx.x] = loss;
+  const int64_t j = n * 4 + t;
+  if (t < 4 && j < s.steps && (!m || m[j])) v += (double)a[j] - (r ? (double)r[j] : 0.0);
+  return v;
+}
+struct PairIo {
+  Side w, l;
+  int64_t pairs;
+  double beta, eps, scale;      // scale: 1 / pairs of the mean included
+  float *margin, *coef, *loss;
+  double* part;
+};
+// TPP threads per pair: a wave where the sequences are short, a block where they are long.
+template <int TPP> __global__ void __launch_bounds__(256) k_pairs(PairIo io) {
+  __shared__ double sd[4];
+  const int t = threadIdx.x % TPP;
+  double loss = 0.0;
+  for (int64_t p = (int64_t)blockIdx.x * (256 / TPP) + threadIdx.x / TPP; p < io.pairs; p += (int64_t)gridDim.x * (256 / TPP)) {
+    double h = side_sum<TPP>(io.w, p, t) - side_sum<TPP>(io.l, p, t);
+    h = TPP == 64 ? wave_sum(h) : block_sum<256>(h, sd);
+    if (t == 0) {
+      const double z = io.beta * h, e = exp(-fabs(z)), lp = log1p(e);
+      const double neg = (z < 0.0 ? -z : 0.0) + lp, pos = (z > 0.0 ? z : 0.0) + lp;      // -ln sigmoid(z), -ln sigmoid(-z)
+      const double small = e / (1.0 + e), big = 1.0 / (1.0 + e), up = z >= 0.0 ? big : small, down = z >= 0.0 ? small : big;   // sigmoid(z), sigmoid(-z)
+      io.margin[p] = (float)z;
+      io.coef[p] = (float)(io.scale * io.beta * (io.eps * up - (1.0 - io.eps) * down));
+      loss += z != z ? z : (1.0 - io.eps) * neg + io.eps * pos;
+    }
+  }
+  loss = block_sum<256>(loss, sd);
+  if (threadIdx.x) return;
+  if (gridDim.x > 1) io.part[blockIdx.x] = loss;
+  else *io.loss = (float)(loss * io.scale);       // (a launch of one block has the whole sum)
 }
 __global__ void __launch_bounds__(256) k_pairs_finish(const double* part, int blocks, double scale, float* out) {
   __shared__ double sd[4];
-  double v = 0.0;
-  for (int b = threadIdx.x; b < blocks; b += 256) v += part[b];
-  v = block_sum<256>(v, sd);
+  const double v = block_sum<256>(long_sum<256>(part, blocks, 1), sd);
   if (threadIdx.x == 0) *out = (float)(v * scale);
 }
-__global__ void __launch_bounds__(256) k_pairs_grad(const float* coef, const float* gain, const uint8_t* mask, int64_t pairs, int64_t steps, float sign, float* out) {
-  const float g = sign * *gain;
-  for (int64_t j = blockIdx.x * 256 + threadIdx.x; j < pairs * steps; j += (int64_t)gridDim.x * 256)
-    out[j] = mask && !mask[j] ? 0.0f : coef[j / steps] * g;
+constexpr int64_t kPairPiece = 1024;      // steps a wave writes
+struct GradSide { float* out; const uint8_t* mask; int64_t steps, pieces; float sign; };
+// Waves over (pair, piece of its steps), the better side's before the worse side's.
+__global__ void __launch_bounds__(256) k_pairs_grad(const float* coef, const float* gain, int64_t pairs, GradSide b, GradSide w) {
+  const float g = *gain;
+  const int lane = threadIdx.x & 63;
+  const int64_t total = pairs * (b.pieces + w.pieces);
+  for (int64_t u = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; u < total; u += (int64_t)gridDim.x * 4) {
+    const bool first = u < pairs * b.pieces;
+    const GradSide& s = first ? b : w;
+    const int64_t v = first ? u : u - pairs * b.pieces, p = v / s.pieces, j0 = (v - p * s.pieces) * kPairPiece, j1 = min(j0 + kPairPiece, s.steps);
+    const float c = coef[p] * g * s.sign;
+    float* out = s.out + p * s.steps;
+    const uint8_t* m = s.mask ? s.mask + p * s.steps : nullptr;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t j = j0 + (q * 64 + lane) * 4;
+      if (j + 4 <= j1) {
+        const uint32_t keep = m ? ((const Bytes4*)(m + j))->w : 0xffffffffu;
+        Reg<float> x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.w[i] = keep >> 8 * i & 255u ? __float_as_uint(c) : 0u;
+        x.store(out + j);
+      } else {
+        for (int64_t i = j; i < j1; ++i) out[i] = !m || m[i] ? c : 0.0f;
+      }
+    }
+  }
 }
 
 // ---- gradient lists --------------------------------------------------------------------------------------------------------
@@ -692,9 +755,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_clip_norm(ClipTab
 }
 __global__ void __launch_bounds__(1024) k_clip_finish(const double* part, int64_t blocks, double max_norm, double eps, float* norm, float* coef) {
   __shared__ double sd[16];
-  double v = 0.0;
-  for (int64_t b = threadIdx.x; b < blocks; b += 1024) v += part[b];
-  v = block_sum<1024>(v, sd);
+  const double v = block_sum<1024>(long_sum<1024>(part, blocks, 1), sd);
   if (threadIdx.x == 0) {
     const double n = sqrt(v), c = isinf(max_norm) ? 1.0 : max_norm / (n + eps);
     *norm = (float)n;
@@ -775,7 +836,7 @@ RowPlan plan_rows(int64_t rows, int64_t k, int size) {
   auto grid = [&](int64_t per_block, int64_t most) { const int64_t b = (rows + per_block - 1) / per_block; return b < most ? b : most; };
   if (k <= kShort) {
     const int g = k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : k <= 64 ? 16 : k <= 128 ? 32 : 64;
-    p.grid = rows * k <= 4096 ? 1 : grid(256 / g, kMaxGrid);
+    p.grid = rows <= 2 * 256 / g ? 1 : grid(256 / g, kMaxGrid);      // (two turns of one block cost less than the launch that joins blocks)
   } else if (rows <= 128 && bytes >= 32768) {
     p.kind = 3;
     const int64_t want = 512 / rows, most = bytes / 8192;
@@ -930,21 +991,25 @@ extern "C" int ps_preference_loss(const ps_preference* q, float* loss, float* ma
   if (!std::isfinite(q->beta) || !(q->label_smoothing >= 0.0 && q->label_smoothing <= 1.0) || !std::isfinite(q->scale)) return set_error(PS_E_ARG, "ps_preference_loss: beta and scale must be finite, label_smoothing in [0, 1]");
   if (int e = check_space(workspace, workspace_bytes, ps_preference_loss_workspace(q->pairs), "ps_preference_loss")) return e;
   Launches run{(hipStream_t)stream};
-  const int grid = block_grid(q->pairs);
   const double scale = q->scale / (q->mean ? (double)q->pairs : 1.0);
-  run(k_pairs, grid, 256, Side{q->better, q->better_ref, q->better_mask, q->better_steps}, Side{q->worse, q->worse_ref, q->worse_mask, q->worse_steps},
-                                                 q->pairs, q->beta, q->label_smoothing, scale, margin, coef, (double*)workspace);
-  run(k_pairs_finish, 1, 256, (const double*)workspace, grid, scale, loss);
+  const PairIo io{Side{q->better, q->better_ref, q->better_mask, q->better_steps}, Side{q->worse, q->worse_ref, q->worse_mask, q->worse_steps}, q->pairs, q->beta, q->label_smoothing,
+                  scale, margin, coef, loss, (double*)workspace};
+  // a wave per pair up to 512 steps of its longer side, a block beyond; 16 such waves' pairs or less are one block's, which then needs no second launch
+  const bool wave = (q->better_steps > q->worse_steps ? q->better_steps : q->worse_steps) <= 512;
+  const int grid = wave ? (q->pairs <= 16 ? 1 : block_grid((q->pairs + 3) / 4)) : block_grid(q->pairs);
+  if (wave) run(k_pairs<64>, grid, 256, io);
+  else run(k_pairs<256>, grid, 256, io);
+  if (grid > 1) run(k_pairs_finish, 1, 256, (const double*)workspace, grid, scale, loss);
   return run.result("ps_preference_loss");
 }
 
 extern "C" int ps_preference_grad(const ps_preference* q, const float* coef, const float* gain, float* better_grad, float* worse_grad, void* stream) {
   if (!q || q->pairs < 1 || q->better_steps < 0 || q->worse_steps < 0 || !coef || !gain) return set_error(PS_E_ARG, "ps_preference_grad: bad pairs, or NULL coef or gain");
   Launches run{(hipStream_t)stream};
-  const int64_t nb = q->pairs * q->better_steps, nw = q->pairs * q->worse_steps;
-  auto grid = [](int64_t n) { const int64_t b = (n + 255) / 256; return (int)(b < kMaxGrid ? b : kMaxGrid); };
-  if (better_grad && nb) run(k_pairs_grad, grid(nb), 256, coef, gain, q->better_mask, q->pairs, q->better_steps, 1.0f, better_grad);
-  if (worse_grad && nw) run(k_pairs_grad, grid(nw), 256, coef, gain, q->worse_mask, q->pairs, q->worse_steps, -1.0f, worse_grad);
+  auto side = [&](float* out, const uint8_t* mask, int64_t steps, float sign) { return GradSide{out, mask, steps, out ? (steps + kPairPiece - 1) / kPairPiece : 0, sign}; };
+  const GradSide b = side(better_grad, q->better_mask, q->better_steps, 1.0f), w = side(worse_grad, q->worse_mask, q->worse_steps, -1.0f);
+  const int64_t units = q->pairs * (b.pieces + w.pieces);
+  if (units) run(k_pairs_grad, block_grid((units + 3) / 4), 256, coef, gain, q->pairs, b, w);
   return run.result("ps_preference_grad");
 }
 
