@@ -117,6 +117,7 @@ __device__ __forceinline__ RowLoss row_loss(const Policy& p, int64_t i, double l
   return o;
 }
 constexpr int LOGP = 0, POLICY = 1;
+constexpr int GRAD_NONE = 0, GRAD_KEPT = 1, GRAD_PAST = 2;      // no gradient; one that its reader may find in the caches; one larger than the caches, written past them
 constexpr int kMaxGrid = 2048;        // row blocks of a launch (8 per CU); rows are dealt out in turn
 constexpr int64_t kCountInline = 1024;   // masks up to this many rows are counted by every block itself, longer ones by a launch of their own
 
@@ -136,17 +137,25 @@ struct RowIo {
 template <typename T> struct Reg {
   static constexpr int N = 16 / sizeof(T);
   uint32_t w[4];
-  struct __attribute__((packed, aligned(sizeof(T)))) Mem { uint32_t w[4]; };
+  typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));      // (element-aligned; the attribute takes no expression of T)
   __device__ __forceinline__ void load(const T* p) {
-    const Mem m = *(const Mem*)p;
+    const Words m = *(const Words*)p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = m.w[i];
+    for (int i = 0; i < 4; ++i) w[i] = m[i];
   }
   __device__ __forceinline__ void store(T* p) const {
-    Mem m;
+    const Words m = {w[0], w[1], w[2], w[3]};
+    *(Words*)p = m;
+  }
+  // the same past the caches, for what nobody reads again soon
+  __device__ __forceinline__ void load_once(const T* p) {
+    const Words m = __builtin_nontemporal_load((const Words*)p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m.w[i] = w[i];
-    *(Mem*)p = m;
+    for (int i = 0; i < 4; ++i) w[i] = m[i];
+  }
+  __device__ __forceinline__ void store_once(T* p) const {
+    const Words m = {w[0], w[1], w[2], w[3]};
+    __builtin_nontemporal_store(m, (Words*)p);
   }
   // the packed words are what lives from one use to the next: without this the compiler keeps the 32-bit elements of the first use (twice the
   // registers, 128 - 2000 B of scratch per lane in the widest kernels)
@@ -284,7 +293,7 @@ template <int THREADS> __device__ __forceinline__ void end_block(const RowIo& io
 }
 
 // Short rows: G lanes hold a row, N elements each.
-template <typename T, int G, int N, int MODE, bool GRAD> __global__ void __launch_bounds__(256) k_rows_short(RowIo io) {
+template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch_bounds__(256) k_rows_short(RowIo io) {
   __shared__ double sd[4];
   double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
   int64_t count = 0;
@@ -335,13 +344,28 @@ template <typename T, int G, int N, int MODE, bool GRAD> __global__ void __launc
   if (MODE == POLICY) end_block<256>(io, blockIdx.x, acc, count, weight, sd);
 }
 
-// one 16-byte piece of a row's gradient, -coef e^(x - m) inv; the chosen element's share of coef is added behind it (chosen_element)
-template <typename T> __device__ __forceinline__ void grad_piece(Reg<T>& v, float m, float scale) {
+// One 16-byte piece of a row's gradient, -coef e^(x - m) inv; the chosen element's share of coef is added behind it (chosen_element).  16-bit results
+// take the factor into the exponent, |scale| e^d = 2^(d log2 e + log2 |scale|), and its sign afterwards: 6 instead of 8 operations an element beside the
+// exponential, at most (|d| + |log2 scale|) 2^-23 relative, a hundredth of their half step.
+struct GradScale {
+  float m, scale, log2_scale;
+  uint32_t sign;
+  __device__ __forceinline__ GradScale(float m_, float scale_) : m(m_), scale(scale_), log2_scale(__builtin_amdgcn_logf(fabsf(scale_))), sign(__float_as_uint(scale_) >> 31 ? 0x80008000u : 0u) {}
+};
+template <typename T> __device__ __forceinline__ void grad_piece(Reg<T>& v, const GradScale& s) {
   float f[Reg<T>::N];
   v.get(f);
+  if (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < Reg<T>::N; ++i) f[i] = exp_of<T>(f[i] - m) * scale;
-  v.set(f);
+    for (int i = 0; i < Reg<T>::N; ++i) f[i] = exp_of<T>(f[i] - s.m) * s.scale;
+    v.set(f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Reg<T>::N; ++i) f[i] = __builtin_amdgcn_exp2f(fmaf(f[i] - s.m, 1.44269502e+0f, s.log2_scale));
+    v.set(f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.w[i] ^= s.sign;
+  }
 }
 // Thread t of TPR owns the piece the chosen column c lies in (pieces of V elements dealt out in turn from column j0, a tail of single elements behind
 // the last whole one): it writes that element once more, whole.
@@ -361,7 +385,7 @@ template <typename T, int THREADS> __device__ __forceinline__ void zero_row(T* d
 
 // Rows that fit the registers of WAVES waves, NV 16-byte pieces per thread: one read of the row for its statistics and its gradient.  One row per
 // group of waves and no loop over rows: inside a loop the compiler would hold the 64-bit functions' constants in 40 registers all the time.
-template <typename T, int WAVES, int NV, int MODE, bool GRAD> __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) k_rows_held(RowIo io) {
+template <typename T, int WAVES, int NV, int MODE, int GRAD> __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) k_rows_held(RowIo io) {
   constexpr int THREADS = WAVES == 1 ? 256 : WAVES * 64, TPR = WAVES * 64, V = Reg<T>::N;
   __shared__ double sd[THREADS / 64];
   __shared__ Part joined[WAVES];
@@ -383,7 +407,7 @@ template <typename T, int WAVES, int NV, int MODE, bool GRAD> __global__ void __
       Reg<T> v[NV];
 #pragma unroll
       for (int q = 0; q < NV; ++q)
-        if (q * TPR + t < nv) v[q].load(x + q * (TPR * V) + (uint32_t)(t * V));
+        if (q * TPR + t < nv) v[q].load_once(x + q * (TPR * V) + (uint32_t)(t * V));
       const int64_t tail = (int64_t)nv * V + t;
       const float last = t < rest ? to_f32(x[tail]) : -INFINITY;
       const int64_t c = choice_of(r, i);
@@ -423,12 +447,14 @@ template <typename T, int WAVES, int NV, int MODE, bool GRAD> __global__ void __
       const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, t == 0, acc);
       if (GRAD) {
         const float scale = -e.coef * e.inv;
+        const GradScale gs(a.m, scale);
 #pragma unroll
         for (int q = 0; q < NV; ++q)
           if (q * TPR + t < nv) {
             v[q].forget();
-            grad_piece<T>(v[q], a.m, scale);
-            v[q].store(dx + q * (TPR * V) + (uint32_t)(t * V));
+            grad_piece<T>(v[q], gs);
+            if (GRAD == GRAD_PAST) v[q].store_once(dx + q * (TPR * V) + (uint32_t)(t * V));
+            else v[q].store(dx + q * (TPR * V) + (uint32_t)(t * V));
             __builtin_amdgcn_sched_barrier(0);
           }
         if (t < rest) dx[tail] = from_f32<T>(exp_of<T>(last - a.m) * scale);
@@ -439,35 +465,50 @@ template <typename T, int WAVES, int NV, int MODE, bool GRAD> __global__ void __
   if (MODE == POLICY) end_block<THREADS>(io, block, acc, count, weight, sd);
 }
 
-// (maximum, sum) of the elements [j0, j1) of a row by one block, in one pass: every thread keeps its running maximum and rescales its sum when it
-// grows.  j0 is a multiple of 16 bytes' worth of elements; THREADS a power of two of waves.
+// (maximum, sum) of the elements [j0, j1) of a row by one block, in one pass, four pieces in flight per thread: every thread keeps its running maximum
+// and rescales its sum when it grows.  THREADS a power of two of waves.
 template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(const T* x, int64_t j0, int64_t j1, Part* slots) {
-  constexpr int V = Reg<T>::N;
+  constexpr int V = Reg<T>::N, U = 4;
   Part a{0.0, -INFINITY};
   const int64_t n = (j1 - j0) / V;
-  auto take = [&](const float* f, int cnt) {
-    float m = f[0];
-    for (int j = 1; j < cnt; ++j) m = fmaxf(m, f[j]);
+  auto raise = [&](float m) {
     if (m > a.m) {
       if (a.s != 0.0) a.s *= (double)exp_of<T>(a.m - m);      // (nothing yet, or -inf alone: 0 stays 0)
       a.m = m;
     }
-    const float base = base_of(a.m);
-    float e = 0.0f;
-    for (int j = 0; j < cnt; ++j) e += exp_of<T>(f[j] - base);
-    a.s += (double)e;
   };
-  for (int64_t q = threadIdx.x; q < n; q += THREADS) {
-    Reg<T> v;
-    v.load(x + j0 + q * V);
-    float f[V];
-    v.get(f);
-    take(f, V);
+  for (int64_t q = threadIdx.x; q < n; q += U * THREADS) {
+    Reg<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q + u * THREADS < n) v[u].load(x + j0 + (q + u * THREADS) * V);
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q + u * THREADS < n) {
+        float f[V];
+        v[u].get(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, f[j]);
+      }
+    raise(m);
+    const float base = base_of(a.m);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q + u * THREADS < n) {
+        float f[V], e = 0.0f;
+        v[u].forget();
+        v[u].get(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) e += exp_of<T>(f[j] - base);
+        a.s += (double)e;
+      }
   }
   const int64_t tail = j0 + n * V + threadIdx.x;
   if (tail < j1) {
     const float f = to_f32(x[tail]);
-    take(&f, 1);
+    raise(f);
+    a.s += (double)exp_of<T>(f - base_of(a.m));
   }
   a = join_lanes<64>(a);
   __syncthreads();
@@ -479,10 +520,11 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
 template <typename T, int THREADS> __device__ __forceinline__ void stream_grad(const T* x, T* dx, int64_t j0, int64_t j1, float m, float scale, float coef, int64_t c, float xc) {
   constexpr int V = Reg<T>::N;
   const int64_t n = (j1 - j0) / V;
+  const GradScale gs(m, scale);
   for (int64_t q = threadIdx.x; q < n; q += THREADS) {
     Reg<T> v;
-    v.load(x + j0 + q * V);
-    grad_piece<T>(v, m, scale);
+    v.load_once(x + j0 + q * V);
+    grad_piece<T>(v, gs);
     v.store(dx + j0 + q * V);
   }
   const int64_t tail = j0 + n * V + threadIdx.x;
@@ -490,30 +532,30 @@ template <typename T, int THREADS> __device__ __forceinline__ void stream_grad(c
   chosen_element<T, THREADS>(dx, j0, j1, c, threadIdx.x, xc, m, scale, coef);
 }
 
-// Rows longer than the registers of a block: a pass for the statistics, a second one for the gradient.
-template <typename T, int MODE, bool GRAD> __global__ void __launch_bounds__(1024) k_rows_long(RowIo io) {
-  __shared__ double sd[16];
-  __shared__ Part slots[16];
+// Rows longer than the registers of a block: a pass for the statistics, a second one for the gradient.  One row per block (see k_rows_held).
+template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(512) k_rows_long(RowIo io) {
+  __shared__ double sd[8];
+  __shared__ Part slots[8];
+  const int64_t i = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (i >= io.r.rows) return;      // (the last line of a two-dimensional grid)
   double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
   int64_t count = 0;
-  if (MODE == POLICY) weight = weight_of<1024>(io, &count, sd);
+  if (MODE == POLICY) weight = weight_of<512>(io, &count, sd);
   const Rows& r = io.r;
-  for (int64_t i = blockIdx.x; i < r.rows; i += gridDim.x) {
-    T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
-    if (r.mask && !r.mask[i]) {
-      if (threadIdx.x == 0) masked_row(io, i);
-      if (GRAD) zero_row<T, 1024>(dx, r.k, threadIdx.x);
-      continue;
-    }
+  T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
+  if (r.mask && !r.mask[i]) {
+    if (threadIdx.x == 0) masked_row(io, i);
+    if (GRAD) zero_row<T, 512>(dx, r.k, threadIdx.x);
+  } else {
     const T* x = (const T*)r.x + i * r.stride;
     const int64_t c = choice_of(r, i);
     const bool ok = c >= 0 && c < r.k;
     const float xc = to_f32(x[ok ? c : 0]);
-    const Part a = stream_part<T, 1024>(x, 0, r.k, slots);
+    const Part a = stream_part<T, 512>(x, 0, r.k, slots);
     const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, threadIdx.x == 0, acc);
-    if (GRAD) stream_grad<T, 1024>(x, dx, 0, r.k, a.m, -e.coef * e.inv, e.coef, c, xc);
+    if (GRAD) stream_grad<T, 512>(x, dx, 0, r.k, a.m, -e.coef * e.inv, e.coef, c, xc);
   }
-  if (MODE == POLICY) end_block<1024>(io, blockIdx.x, acc, count, weight, sd);
+  if (MODE == POLICY) end_block<512>(io, i, acc, count, weight, sd);
 }
 
 // Few long rows: `splits` blocks share a row (at most 64), `step` elements each.  First launch: the blocks' (maximum, sum) ...
@@ -525,7 +567,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_split_part(Rows r
   if (threadIdx.x == 0) out[blockIdx.x] = a;
 }
 // ... second launch: joined by every block for its own stretch of the gradient; the row's first block writes what belongs to the row.
-template <typename T, int MODE, bool GRAD> __global__ void __launch_bounds__(256) k_split_end(RowIo io, int splits, int64_t step, const Part* parts, int blocks_per_row) {
+template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(256) k_split_end(RowIo io, int splits, int64_t step, const Part* parts, int blocks_per_row) {
   __shared__ double sd[4];
   double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
   int64_t count = 0;
@@ -736,7 +778,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_clip_norm(ClipTab
 #pragma unroll
   for (int q = 0; q < kClipPieces; ++q) {
     v[q].w[0] = v[q].w[1] = v[q].w[2] = v[q].w[3] = 0;
-    if (q * 256 + (int)threadIdx.x < n) v[q].load(g + q * (256 * V) + threadIdx.x * V);
+    if (q * 256 + (int)threadIdx.x < n) v[q].load_once(g + q * (256 * V) + threadIdx.x * V);
   }
   double a = 0.0;
   if (n * V + (int)threadIdx.x < len) {
@@ -773,7 +815,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_clip_scale(ClipTa
   Reg<T> v[kClipPieces];
 #pragma unroll
   for (int q = 0; q < kClipPieces; ++q)
-    if (q * 256 + (int)threadIdx.x < n) v[q].load(g + q * (256 * V) + threadIdx.x * V);
+    if (q * 256 + (int)threadIdx.x < n) v[q].load_once(g + q * (256 * V) + threadIdx.x * V);
   if (n * V + (int)threadIdx.x < len) {
     T* e = g + n * V + threadIdx.x;
     *e = from_f32<T>(to_f32(*e) * c);
@@ -829,6 +871,7 @@ struct RowPlan {
   int splits;
   int64_t step;
 };
+constexpr int64_t kPastCaches = 256 << 20;      // bytes of the last-level cache
 constexpr int kShort = 256;            // elements a row of k_rows_short may have (64 lanes x 4)
 RowPlan plan_rows(int64_t rows, int64_t k, int size) {
   const int64_t bytes = k * size, pieces = k * size / 16;
@@ -853,21 +896,22 @@ RowPlan plan_rows(int64_t rows, int64_t k, int size) {
     p.grid = rows;
   } else {
     p.kind = 2;
-    p.grid = grid(1, kMaxGrid);
+    p.grid = rows;
   }
   return p;
 }
-template <typename T, int MODE, bool GRAD> void launch_rows(Launches& run, const RowIo& io, const RowPlan& p, Part* parts) {
+template <typename T, int MODE, int GRAD> void launch_rows(Launches& run, const RowIo& io, const RowPlan& p, Part* parts) {
   const int64_t k = io.r.k, pieces = k / Reg<T>::N;
   const int wide = 1 << 16;
   const dim3 rows2d(p.grid < wide ? (int)p.grid : wide, (int)((p.grid + wide - 1) / wide));
+  constexpr int G1 = GRAD == GRAD_PAST ? GRAD_KEPT : GRAD;       // (the kernels that make no difference)
   if (p.kind == 0) {
-    if (k <= 4) run(k_rows_short<T, 4, 1, MODE, GRAD>, (int)p.grid, 256, io);
-    else if (k <= 8) run(k_rows_short<T, 8, 1, MODE, GRAD>, (int)p.grid, 256, io);
-    else if (k <= 16) run(k_rows_short<T, 16, 1, MODE, GRAD>, (int)p.grid, 256, io);
-    else if (k <= 64) run(k_rows_short<T, 16, 4, MODE, GRAD>, (int)p.grid, 256, io);
-    else if (k <= 128) run(k_rows_short<T, 32, 4, MODE, GRAD>, (int)p.grid, 256, io);
-    else run(k_rows_short<T, 64, 4, MODE, GRAD>, (int)p.grid, 256, io);
+    if (k <= 4) run(k_rows_short<T, 4, 1, MODE, G1>, (int)p.grid, 256, io);
+    else if (k <= 8) run(k_rows_short<T, 8, 1, MODE, G1>, (int)p.grid, 256, io);
+    else if (k <= 16) run(k_rows_short<T, 16, 1, MODE, G1>, (int)p.grid, 256, io);
+    else if (k <= 64) run(k_rows_short<T, 16, 4, MODE, G1>, (int)p.grid, 256, io);
+    else if (k <= 128) run(k_rows_short<T, 32, 4, MODE, G1>, (int)p.grid, 256, io);
+    else run(k_rows_short<T, 64, 4, MODE, G1>, (int)p.grid, 256, io);
   } else if (p.kind == 1) {
     if (pieces <= 128) run(k_rows_held<T, 1, 2, MODE, GRAD>, rows2d, 256, io);
     else if (pieces <= 512) run(k_rows_held<T, 1, 8, MODE, GRAD>, rows2d, 256, io);
@@ -877,11 +921,11 @@ template <typename T, int MODE, bool GRAD> void launch_rows(Launches& run, const
     else if (pieces <= 8192) run(k_rows_held<T, 16, 8, MODE, GRAD>, rows2d, 1024, io);
     else run(k_rows_held<T, 16, 16, MODE, GRAD>, rows2d, 1024, io);
   } else if (p.kind == 2) {
-    run(k_rows_long<T, MODE, GRAD>, (int)p.grid, 1024, io);
+    run(k_rows_long<T, MODE, G1>, rows2d, 512, io);
   } else {
     run(k_split_part<T>, (int)p.grid, 256, io.r, p.splits, p.step, parts);
     const int per_row = GRAD ? p.splits : 1;
-    run(k_split_end<T, MODE, GRAD>, (int)(io.r.rows * per_row), 256, io, p.splits, p.step, (const Part*)parts, per_row);
+    run(k_split_end<T, MODE, G1>, (int)(io.r.rows * per_row), 256, io, p.splits, p.step, (const Part*)parts, per_row);
   }
 }
 
@@ -917,7 +961,7 @@ extern "C" int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, v
   by_type(d->dtype, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
     const RowPlan p = plan_rows(io.r.rows, io.r.k, sizeof(T));
-    launch_rows<T, LOGP, false>(run, io, p, RowSpace(workspace, p, io.r.rows).parts);
+    launch_rows<T, LOGP, GRAD_NONE>(run, io, p, RowSpace(workspace, p, io.r.rows).parts);
     return 0;
   });
   return run.result("ps_choice_logp");
@@ -971,12 +1015,14 @@ extern "C" int ps_policy_loss(const ps_decisions* d, const ps_policy_terms* q, f
   io.loss = loss;
   io.kl = kl;
   io.clip_frac = clip_frac;
+  const bool past = r.rows * r.k * (d->dtype == PS_F32 ? 4 : 2) >= kPastCaches;
   if (counted) run(k_count, 1, 1024, r.mask, r.rows, w.count);
   if (r.rows)
     by_type(d->dtype, [&](auto* t) {
       typedef std::remove_pointer_t<decltype(t)> T;
-      if (grad) launch_rows<T, POLICY, true>(run, io, p, w.parts);
-      else launch_rows<T, POLICY, false>(run, io, p, w.parts);
+      if (grad && past && p.kind == 1) launch_rows<T, POLICY, GRAD_PAST>(run, io, p, w.parts);
+      else if (grad) launch_rows<T, POLICY, GRAD_KEPT>(run, io, p, w.parts);
+      else launch_rows<T, POLICY, GRAD_NONE>(run, io, p, w.parts);
       return 0;
     });
   if (p.grid != 1 || p.kind == 3) run(k_policy_finish, 1, 256, io, p.kind == 3 ? r.rows : p.grid);      // (a launch of one block has written the results itself)
