@@ -32,13 +32,44 @@ template <typename T> __device__ __forceinline__ float exp_of(float d) {
 }
 template <> __device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
 
+// The few 64-bit functions a row needs at its end, to about 1e-11 relative -- far beyond what its sum of exponentials carries -- in a quarter of the
+// library's instructions (a wave spends as long on the library's log, exp and expm1 as on 1500 elements) and without its 40 registers of constants.
+// exp: a = n ln 2 + f, |f| <= 0.35, Taylor's series to f^10 / 10!.  NaN stays, overflow is inf, underflow 0.
+__device__ __forceinline__ double exp64(double a) {
+  a = a > 800.0 ? 800.0 : a;
+  a = a < -800.0 ? -800.0 : a;
+  const double n = rint(a * 1.4426950408889634);
+  const double f = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, a));      // ln 2 in two parts, the first with 21 zero bits behind
+  double p = 1.0 / 3628800.0;
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return ldexp(p, (int)n);
+}
+// ln s for a finite s >= 2^-100: y = the 32-bit logarithm, then one step with s e^-y = 1 + r, ln s = y + r - r^2 / 2 + r^3 / 3, |r| < 1e-5.
+__device__ __forceinline__ double log64(double s) {
+  const double y = (double)(__builtin_amdgcn_logf((float)s) * 0.693147180559945f);
+  const double r = fma(s, exp64(-y), -1.0);
+  return y + r * fma(r, fma(r, 1.0 / 3.0, -0.5), 1.0);
+}
+
 // ---- block reductions (fixed order) ----------------------------------------------------------------------------------------
-__device__ __forceinline__ double wave_sum(double v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+// over groups of G neighbouring lanes (a power of two), every lane gets the result
+template <int G = 64> __device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+template <int G = 64> __device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   return v;
 }
 // sum over the block, the same value in every thread; `s` holds one double per wave and may be reused after the call
@@ -97,7 +128,7 @@ struct Policy {
 struct RowLoss { double loss, kl, clip, d_logp; };
 __device__ __forceinline__ RowLoss row_loss(const Policy& p, int64_t i, double logp) {
   RowLoss o;
-  const double adv = p.advantage[i], r = exp(logp - (double)p.old_logp[i]);
+  const double adv = p.advantage[i], r = exp64(logp - (double)p.old_logp[i]);
   // (comparisons written so that a NaN ratio or advantage stays NaN: fmin / fmax would drop it)
   const double rc = r < p.lo ? p.lo : (r > p.hi ? p.hi : r);
   const double s1 = r * adv, s2 = rc * adv;
@@ -107,7 +138,7 @@ __device__ __forceinline__ RowLoss row_loss(const Policy& p, int64_t i, double l
   o.clip = clipped ? 1.0 : 0.0;
   o.kl = 0.0;
   if (p.ref_logp) {
-    const double d = (double)p.ref_logp[i] - logp, em1 = expm1(d);
+    const double d = (double)p.ref_logp[i] - logp, em1 = exp64(d) - 1.0;
     o.kl = em1 - d;
     if (p.beta != 0.0) {
       o.loss += p.beta * o.kl;
@@ -209,13 +240,9 @@ struct Part { double s; float m; };
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 // join the parts of a group of lanes (G a power of two); every lane gets the result
 template <int G> __device__ __forceinline__ Part join_lanes(Part a) {
-  float m = a.m;
-#pragma unroll
-  for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  double s = a.s == 0.0 ? 0.0 : a.s * exp((double)a.m - (double)m);      // (NaN sums stay NaN: NaN == 0 is false)
-#pragma unroll
-  for (int o = G / 2; o; o >>= 1) s += __shfl_xor(s, o);
-  return Part{s, m};
+  const float m = wave_max<G>(a.m);
+  const double s = a.s == 0.0 ? 0.0 : a.s * exp64((double)a.m - (double)m);      // (NaN sums stay NaN: NaN == 0 is false)
+  return Part{wave_sum<G>(s), m};
 }
 
 __device__ __forceinline__ int nonzero_bytes(const Reg<uint8_t>& q) {
@@ -252,9 +279,9 @@ template <int THREADS> __device__ __forceinline__ double weight_of(const RowIo& 
 // What a row's statistics make of it: log-probability, loss terms, the coefficient of its gradient.  Every lane of the row's group calls it.
 struct RowEnd { float coef, inv; };
 template <int MODE> __device__ __forceinline__ RowEnd end_row(const RowIo& io, int64_t i, int64_t c, bool ok, float xc, Part a, double weight, bool writer, double* acc) {
-  const double logp = ok ? ((double)xc - (double)a.m) - log(a.s) : (double)NAN;
+  const double logp = ok ? ((double)xc - (double)a.m) - log64(a.s) : (double)NAN;
   RowEnd e;
-  e.inv = ok ? (float)(1.0 / a.s) : NAN;      // (a choice outside the row makes its gradient NaN too)
+  e.inv = ok ? 1.0f / (float)a.s : NAN;      // (a choice outside the row makes its gradient NaN too)
   e.coef = 0.0f;
   if (MODE == POLICY) {
     const RowLoss o = row_loss(io.p, i, logp);
@@ -321,8 +348,7 @@ template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch
       f[q] = q * G + lane < k ? to_f32(x[q * G + lane]) : -INFINITY;
       a.m = fmaxf(a.m, f[q]);
     }
-#pragma unroll
-    for (int o = G / 2; o; o >>= 1) a.m = fmaxf(a.m, __shfl_xor(a.m, o));
+    a.m = wave_max<G>(a.m);
     const float base = base_of(a.m);
     float t = 0.0f;
 #pragma unroll
@@ -330,9 +356,7 @@ template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch
       f[q] = exp_of<T>(f[q] - base);
       t += f[q];
     }
-    a.s = (double)t;
-#pragma unroll
-    for (int o = G / 2; o; o >>= 1) a.s += __shfl_xor(a.s, o);
+    a.s = wave_sum<G>((double)t);
     const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, lane == 0, acc);
     if (GRAD) {
       const float scale = -e.coef * e.inv;
@@ -383,10 +407,12 @@ template <typename T, int THREADS> __device__ __forceinline__ void zero_row(T* d
   if (nv * Reg<T>::N + t < k && t < Reg<T>::N) dx[nv * Reg<T>::N + t] = from_f32<T>(0.0f);
 }
 
-// Rows that fit the registers of WAVES waves, NV 16-byte pieces per thread: one read of the row for its statistics and its gradient.  One row per
-// group of waves and no loop over rows: inside a loop the compiler would hold the 64-bit functions' constants in 40 registers all the time.
-template <typename T, int WAVES, int NV, int MODE, int GRAD> __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) k_rows_held(RowIo io) {
-  constexpr int THREADS = WAVES == 1 ? 256 : WAVES * 64, TPR = WAVES * 64, V = Reg<T>::N;
+// Rows that fit the registers of TPR threads (8 .. 64 lanes of a wave, or that many waves of a block), NV 16-byte pieces per thread: one read of the
+// row for its statistics and its gradient.  One row per group and no loop over rows: inside a loop the compiler would keep the 64-bit functions'
+// constants in registers all the time.
+template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_rows_held(RowIo io) {
+  constexpr int THREADS = TPR <= 64 ? 256 : TPR, WAVES = TPR <= 64 ? 1 : TPR / 64, LANES = TPR < 64 ? TPR : 64, V = Reg<T>::N;
+  static_assert(TPR >= V, "the elements behind the last whole piece have a thread each");
   __shared__ double sd[THREADS / 64];
   __shared__ Part joined[WAVES];
   const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
@@ -396,10 +422,11 @@ template <typename T, int WAVES, int NV, int MODE, int GRAD> __global__ void __l
   if (MODE == POLICY) weight = weight_of<THREADS>(io, &count, sd);
   const Rows& r = io.r;
   const int t = threadIdx.x % TPR, nv = (int)(r.k / V), rest = (int)(r.k - (int64_t)nv * V);
-  const int64_t i = block * (THREADS / TPR) + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);    // (a wave has one row: its addresses live in scalar registers)
+  // (where a wave has one row, its addresses live in scalar registers)
+  const int64_t i = block * (THREADS / TPR) + (TPR < 64 ? (int)threadIdx.x / TPR : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR));
   if (i < r.rows) {
     T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
-    if (r.mask && !r.mask[i]) {        // (uniform over the row's threads)
+    if (r.mask && !r.mask[i]) {        // (the same for all of the row's threads)
       if (t == 0) masked_row(io, i);
       if (GRAD) zero_row<T, TPR>(dx, r.k, t);
     } else {
@@ -422,7 +449,7 @@ template <typename T, int WAVES, int NV, int MODE, int GRAD> __global__ void __l
 #pragma unroll
           for (int j = 0; j < V; ++j) a.m = fmaxf(a.m, f[j]);
         }
-      a.m = wave_max(a.m);
+      a.m = wave_max<LANES>(a.m);
       const float base = base_of(a.m);
       a.s = (double)exp_of<T>(last - base);
 #pragma unroll
@@ -436,7 +463,7 @@ template <typename T, int WAVES, int NV, int MODE, int GRAD> __global__ void __l
           a.s += (double)e;          // (eight terms in 32 bits, then 64)
           __builtin_amdgcn_sched_barrier(0);
         }
-      a.s = wave_sum(a.s);
+      a.s = wave_sum<LANES>(a.s);
       if (WAVES > 1) {
         const int lane = threadIdx.x & 63;
         if (lane == 0) joined[threadIdx.x >> 6] = a;
@@ -872,13 +899,13 @@ struct RowPlan {
   int64_t step;
 };
 constexpr int64_t kPastCaches = 256 << 20;      // bytes of the last-level cache
-constexpr int kShort = 256;            // elements a row of k_rows_short may have (64 lanes x 4)
+constexpr int kShort = 32;             // elements a row of k_rows_short may have
 RowPlan plan_rows(int64_t rows, int64_t k, int size) {
   const int64_t bytes = k * size, pieces = k * size / 16;
   RowPlan p{0, 1, 1, k};
   auto grid = [&](int64_t per_block, int64_t most) { const int64_t b = (rows + per_block - 1) / per_block; return b < most ? b : most; };
   if (k <= kShort) {
-    const int g = k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : k <= 64 ? 16 : k <= 128 ? 32 : 64;
+    const int g = k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : 32;
     p.grid = rows <= 2 * 256 / g ? 1 : grid(256 / g, kMaxGrid);      // (two turns of one block cost less than the launch that joins blocks)
   } else if (rows <= 128 && bytes >= 32768) {
     p.kind = 3;
@@ -890,7 +917,7 @@ RowPlan plan_rows(int64_t rows, int64_t k, int size) {
     p.grid = rows * p.splits;
   } else if (pieces <= 512) {
     p.kind = 1;
-    p.grid = (rows + 3) / 4;
+    p.grid = grid(pieces <= 64 ? 32 : pieces <= 128 ? 16 : pieces <= 256 ? 8 : 4, rows);
   } else if (pieces <= 16384) {
     p.kind = 1;
     p.grid = rows;
@@ -909,17 +936,23 @@ template <typename T, int MODE, int GRAD> void launch_rows(Launches& run, const 
     if (k <= 4) run(k_rows_short<T, 4, 1, MODE, G1>, (int)p.grid, 256, io);
     else if (k <= 8) run(k_rows_short<T, 8, 1, MODE, G1>, (int)p.grid, 256, io);
     else if (k <= 16) run(k_rows_short<T, 16, 1, MODE, G1>, (int)p.grid, 256, io);
-    else if (k <= 64) run(k_rows_short<T, 16, 4, MODE, G1>, (int)p.grid, 256, io);
-    else if (k <= 128) run(k_rows_short<T, 32, 4, MODE, G1>, (int)p.grid, 256, io);
-    else run(k_rows_short<T, 64, 4, MODE, G1>, (int)p.grid, 256, io);
+    else run(k_rows_short<T, 32, 1, MODE, G1>, (int)p.grid, 256, io);
   } else if (p.kind == 1) {
-    if (pieces <= 128) run(k_rows_held<T, 1, 2, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 512) run(k_rows_held<T, 1, 8, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 1024) run(k_rows_held<T, 4, 4, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 2048) run(k_rows_held<T, 4, 8, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 4096) run(k_rows_held<T, 8, 8, MODE, GRAD>, rows2d, 512, io);
-    else if (pieces <= 8192) run(k_rows_held<T, 16, 8, MODE, GRAD>, rows2d, 1024, io);
-    else run(k_rows_held<T, 16, 16, MODE, GRAD>, rows2d, 1024, io);
+    // Threads per row by its pieces.  Few threads with many pieces each beat many with few: the end of a row (64-bit functions, reductions) costs
+    // every wave of it the same (8192-element rows: 1 x 512 rows of 64 threads x 16 pieces 87 us, 2 x 8 89 us, 4 x 4 114 us), and rows that need not
+    // wait for each other overlap one's reading with another's writing (65536-element rows with gradient: 8 waves x 16 pieces 192 us, 16 x 8 251 us).
+    constexpr bool fwd = MODE == LOGP;       // (the policy loss takes the same kernel with and without its gradient: the same bits)
+    if (pieces <= 16) run(k_rows_held<T, 8, 2, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 32) run(k_rows_held<T, 8, 4, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 64) run(k_rows_held<T, 8, 8, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 128) run(k_rows_held<T, 16, 8, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 256) run(k_rows_held<T, 32, 8, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 512) run(k_rows_held<T, 64, 8, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 1024) run(k_rows_held<T, 128, 8, MODE, GRAD>, rows2d, 128, io);
+    else if (pieces <= 2048) run(k_rows_held<T, fwd ? 128 : 256, fwd ? 16 : 8, MODE, GRAD>, rows2d, fwd ? 128 : 256, io);
+    else if (pieces <= 4096) run(k_rows_held<T, 256, 16, MODE, GRAD>, rows2d, 256, io);
+    else if (pieces <= 8192) run(k_rows_held<T, 512, 16, MODE, GRAD>, rows2d, 512, io);
+    else run(k_rows_held<T, 1024, 16, MODE, GRAD>, rows2d, 1024, io);
   } else if (p.kind == 2) {
     run(k_rows_long<T, MODE, G1>, rows2d, 512, io);
   } else {
@@ -976,7 +1009,7 @@ extern "C" int ps_choice_grad(const ps_decisions* d, const float* coef, const fl
   by_type(d->dtype, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
     const float2* st = (const float2*)stat;
-    if (r.k <= kShort) {
+    if (r.k <= 256) {
       const int g = r.k <= 4 ? 4 : r.k <= 16 ? 16 : 64;
       const int64_t b = (r.rows + 256 / g - 1) / (256 / g);
       run(g == 4 ? k_grad_short<T, 4> : g == 16 ? k_grad_short<T, 16> : k_grad_short<T, 64>, (int)(b < kMaxGrid ? b : kMaxGrid), 256, r, coef, st, gain, skip_if_one, (T*)grad);
