@@ -82,16 +82,18 @@ template <int THREADS> __device__ __forceinline__ double block_sum(double v, dou
   for (int i = 0; i < THREADS / 64; ++i) t += s[i];
   return t;
 }
-template <int THREADS> __device__ __forceinline__ float block_max(float v, float* s) {
-  v = wave_max(v);
+// three at once (`s`: three doubles per wave)
+template <int THREADS> __device__ __forceinline__ void block_sum3(double* v, double* s) {
+  for (int q = 0; q < 3; ++q) v[q] = wave_sum(v[q]);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0)
+    for (int q = 0; q < 3; ++q) s[(threadIdx.x >> 6) * 3 + q] = v[q];
   __syncthreads();
-  float t = s[0];
-  for (int i = 1; i < THREADS / 64; ++i) t = fmaxf(t, s[i]);
-  return t;
+  for (int q = 0; q < 3; ++q) {
+    v[q] = 0.0;
+    for (int i = 0; i < THREADS / 64; ++i) v[q] += s[i * 3 + q];
+  }
 }
-
 // sum of n numbers by one block, eight loads in flight per thread
 template <int THREADS> __device__ __forceinline__ double long_sum(const double* part, int64_t n, int64_t stride) {
   double v = 0.0;
@@ -126,9 +128,11 @@ struct Policy {
 
 // what one row contributes: filled by every thread that needs it from the row's statistics
 struct RowLoss { double loss, kl, clip, d_logp; };
-__device__ __forceinline__ RowLoss row_loss(const Policy& p, int64_t i, double logp) {
+struct RowTerms { float old_logp, advantage, ref_logp; };      // (read with the row, long before they are needed)
+__device__ __forceinline__ RowTerms terms_of(const Policy& p, int64_t i) { return RowTerms{p.old_logp[i], p.advantage[i], p.ref_logp ? p.ref_logp[i] : 0.0f}; }
+__device__ __forceinline__ RowLoss row_loss(const Policy& p, const RowTerms& t, double logp) {
   RowLoss o;
-  const double adv = p.advantage[i], r = exp64(logp - (double)p.old_logp[i]);
+  const double adv = t.advantage, r = exp64(logp - (double)t.old_logp);
   // (comparisons written so that a NaN ratio or advantage stays NaN: fmin / fmax would drop it)
   const double rc = r < p.lo ? p.lo : (r > p.hi ? p.hi : r);
   const double s1 = r * adv, s2 = rc * adv;
@@ -138,7 +142,7 @@ __device__ __forceinline__ RowLoss row_loss(const Policy& p, int64_t i, double l
   o.clip = clipped ? 1.0 : 0.0;
   o.kl = 0.0;
   if (p.ref_logp) {
-    const double d = (double)p.ref_logp[i] - logp, em1 = exp64(d) - 1.0;
+    const double d = (double)t.ref_logp - logp, em1 = exp64(d) - 1.0;
     o.kl = em1 - d;
     if (p.beta != 0.0) {
       o.loss += p.beta * o.kl;
@@ -150,7 +154,6 @@ __device__ __forceinline__ RowLoss row_loss(const Policy& p, int64_t i, double l
 constexpr int LOGP = 0, POLICY = 1;
 constexpr int GRAD_NONE = 0, GRAD_KEPT = 1, GRAD_PAST = 2;      // no gradient; one that its reader may find in the caches; one larger than the caches, written past them
 constexpr int kMaxGrid = 2048;        // row blocks of a launch (8 per CU); rows are dealt out in turn
-constexpr int64_t kCountInline = 1024;   // masks up to this many rows are counted by every block itself, longer ones by a launch of their own
 
 // What a launch over rows reads and writes.
 struct RowIo {
@@ -278,13 +281,13 @@ template <int THREADS> __device__ __forceinline__ double weight_of(const RowIo& 
 }
 // What a row's statistics make of it: log-probability, loss terms, the coefficient of its gradient.  Every lane of the row's group calls it.
 struct RowEnd { float coef, inv; };
-template <int MODE> __device__ __forceinline__ RowEnd end_row(const RowIo& io, int64_t i, int64_t c, bool ok, float xc, Part a, double weight, bool writer, double* acc) {
+template <int MODE> __device__ __forceinline__ RowEnd end_row(const RowIo& io, int64_t i, const RowTerms& t, bool ok, float xc, Part a, double weight, bool writer, double* acc) {
   const double logp = ok ? ((double)xc - (double)a.m) - log64(a.s) : (double)NAN;
   RowEnd e;
   e.inv = ok ? 1.0f / (float)a.s : NAN;      // (a choice outside the row makes its gradient NaN too)
   e.coef = 0.0f;
   if (MODE == POLICY) {
-    const RowLoss o = row_loss(io.p, i, logp);
+    const RowLoss o = row_loss(io.p, t, logp);
     e.coef = (float)(o.d_logp * weight);
     if (writer) {
       acc[0] += o.loss;
@@ -304,10 +307,9 @@ __device__ __forceinline__ void masked_row(const RowIo& io, int64_t i) {
   if (io.stat) io.stat[i] = make_float2(0.0f, 0.0f);
   if (io.coef) io.coef[i] = 0.0f;
 }
-// the block's share of the sums -- or, where the launch is one block, the results themselves
-template <int THREADS> __device__ __forceinline__ void end_block(const RowIo& io, int64_t block, const double* acc, int64_t count, double weight, double* sd) {
-  double v[3];
-  for (int q = 0; q < 3; ++q) v[q] = block_sum<THREADS>(acc[q], sd);
+// the block's share of the sums -- or, where the launch is one block, the results themselves.  Where a block has one row, thread 0 has all of it (ONE).
+template <int THREADS, bool ONE> __device__ __forceinline__ void end_block(const RowIo& io, int64_t block, double* v, int64_t count, double weight, double* sd) {
+  if (!ONE) block_sum3<THREADS>(v, sd);
   if (threadIdx.x) return;
   if (gridDim.x > 1 || gridDim.y > 1) {
     for (int q = 0; q < 3; ++q) io.part[block * 3 + q] = v[q];
@@ -321,7 +323,7 @@ template <int THREADS> __device__ __forceinline__ void end_block(const RowIo& io
 
 // Short rows: G lanes hold a row, N elements each.
 template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch_bounds__(256) k_rows_short(RowIo io) {
-  __shared__ double sd[4];
+  __shared__ double sd[12];
   double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
   int64_t count = 0;
   if (MODE == POLICY) weight = weight_of<256>(io, &count, sd);
@@ -341,6 +343,7 @@ template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch
     const int64_t c = choice_of(r, i);
     const bool ok = c >= 0 && c < k;
     const float xc = to_f32(x[ok ? c : 0]);
+    const RowTerms terms = MODE == POLICY ? terms_of(io.p, i) : RowTerms{};
     float f[N];
     Part a{0.0, -INFINITY};
 #pragma unroll
@@ -357,7 +360,7 @@ template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch
       t += f[q];
     }
     a.s = wave_sum<G>((double)t);
-    const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, lane == 0, acc);
+    const RowEnd e = end_row<MODE>(io, i, terms, ok, xc, a, weight, lane == 0, acc);
     if (GRAD) {
       const float scale = -e.coef * e.inv;
 #pragma unroll
@@ -365,7 +368,7 @@ template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch
         if (q * G + lane < k) dx[q * G + lane] = from_f32<T>(fmaf(f[q], scale, q * G + lane == c ? e.coef : 0.0f));
     }
   }
-  if (MODE == POLICY) end_block<256>(io, blockIdx.x, acc, count, weight, sd);
+  if (MODE == POLICY) end_block<256, false>(io, blockIdx.x, acc, count, weight, sd);
 }
 
 // One 16-byte piece of a row's gradient, -coef e^(x - m) inv; the chosen element's share of coef is added behind it (chosen_element).  16-bit results
@@ -413,7 +416,7 @@ template <typename T, int THREADS> __device__ __forceinline__ void zero_row(T* d
 template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_rows_held(RowIo io) {
   constexpr int THREADS = TPR <= 64 ? 256 : TPR, WAVES = TPR <= 64 ? 1 : TPR / 64, LANES = TPR < 64 ? TPR : 64, V = Reg<T>::N;
   static_assert(TPR >= V, "the elements behind the last whole piece have a thread each");
-  __shared__ double sd[THREADS / 64];
+  __shared__ double sd[3 * THREADS / 64];
   __shared__ Part joined[WAVES];
   const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   if (block * (THREADS / TPR) >= io.r.rows) return;      // (the last line of a two-dimensional grid)
@@ -431,15 +434,16 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
       if (GRAD) zero_row<T, TPR>(dx, r.k, t);
     } else {
       const T* x = (const T*)r.x + i * r.stride;
+      const int64_t c = choice_of(r, i);        // (the first load: the chosen logit's address waits for nothing else)
       Reg<T> v[NV];
 #pragma unroll
       for (int q = 0; q < NV; ++q)
         if (q * TPR + t < nv) v[q].load_once(x + q * (TPR * V) + (uint32_t)(t * V));
       const int64_t tail = (int64_t)nv * V + t;
       const float last = t < rest ? to_f32(x[tail]) : -INFINITY;
-      const int64_t c = choice_of(r, i);
       const bool ok = c >= 0 && c < r.k;
       const float xc = to_f32(x[ok ? c : 0]);
+      const RowTerms terms = MODE == POLICY ? terms_of(io.p, i) : RowTerms{};
       Part a{0.0, last};
 #pragma unroll
       for (int q = 0; q < NV; ++q)
@@ -471,7 +475,7 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
         a = joined[lane & (WAVES - 1)];
         a = join_lanes<WAVES>(a);
       }
-      const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, t == 0, acc);
+      const RowEnd e = end_row<MODE>(io, i, terms, ok, xc, a, weight, t == 0, acc);
       if (GRAD) {
         const float scale = -e.coef * e.inv;
         const GradScale gs(a.m, scale);
@@ -489,7 +493,7 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
       }
     }
   }
-  if (MODE == POLICY) end_block<THREADS>(io, block, acc, count, weight, sd);
+  if (MODE == POLICY) end_block<THREADS, (TPR > 64)>(io, block, acc, count, weight, sd);
 }
 
 // (maximum, sum) of the elements [j0, j1) of a row by one block, in one pass, four pieces in flight per thread: every thread keeps its running maximum
@@ -578,11 +582,12 @@ template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(512)
     const int64_t c = choice_of(r, i);
     const bool ok = c >= 0 && c < r.k;
     const float xc = to_f32(x[ok ? c : 0]);
+    const RowTerms terms = MODE == POLICY ? terms_of(io.p, i) : RowTerms{};
     const Part a = stream_part<T, 512>(x, 0, r.k, slots);
-    const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, threadIdx.x == 0, acc);
+    const RowEnd e = end_row<MODE>(io, i, terms, ok, xc, a, weight, threadIdx.x == 0, acc);
     if (GRAD) stream_grad<T, 512>(x, dx, 0, r.k, a.m, -e.coef * e.inv, e.coef, c, xc);
   }
-  if (MODE == POLICY) end_block<512>(io, i, acc, count, weight, sd);
+  if (MODE == POLICY) end_block<512, true>(io, i, acc, count, weight, sd);
 }
 
 // Few long rows: `splits` blocks share a row (at most 64), `step` elements each.  First launch: the blocks' (maximum, sum) ...
@@ -611,11 +616,12 @@ template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(256)
     const int64_t c = choice_of(r, i);
     const bool ok = c >= 0 && c < r.k;
     const float xc = to_f32(x[ok ? c : 0]);
+    const RowTerms terms = MODE == POLICY ? terms_of(io.p, i) : RowTerms{};
     const int lane = threadIdx.x & 63;
     Part a{0.0, -INFINITY};
     if (lane < splits) a = parts[i * splits + lane];
     a = join_lanes<64>(a);
-    const RowEnd e = end_row<MODE>(io, i, c, ok, xc, a, weight, first, acc);
+    const RowEnd e = end_row<MODE>(io, i, terms, ok, xc, a, weight, first, acc);
     if (GRAD) stream_grad<T, 256>(x, dx, j0, j1, a.m, -e.coef * e.inv, e.coef, c, xc);
   }
   if (MODE == POLICY && j0 == 0) {       // (uniform over the block)
@@ -674,36 +680,47 @@ __global__ void __launch_bounds__(1024) k_count(const uint8_t* mask, int64_t n, 
 
 // loss, mean kl, clipped share from the blocks' partial sums
 __global__ void __launch_bounds__(256) k_policy_finish(RowIo io, int64_t blocks) {
-  __shared__ double sd[4];
+  __shared__ double sd[12];
   int64_t count;
   const double weight = weight_of<256>(io, &count, sd);
   double v[3];
   for (int q = 0; q < 3; ++q) v[q] = long_sum<256>(io.part + q, blocks, 3);
-  end_block<256>(io, 0, v, count, weight, sd);
+  end_block<256, false>(io, 0, v, count, weight, sd);
 }
 
 // ---- preference pairs ------------------------------------------------------------------------------------------------------
 struct Side { const float *logp, *ref; const uint8_t* mask; int64_t steps; };
 struct __attribute__((packed)) Bytes4 { uint32_t w; };
-// sum of the log ratios of pair p's valid steps by TPP threads, four steps a piece; masked steps are read with their piece and dropped by selection
+// sum of the log ratios of pair p's valid steps by TPP threads, pieces of four steps, four of them in flight; masked steps are read with their piece
+// and dropped by selection
 template <int TPP> __device__ __forceinline__ double side_sum(const Side& s, int64_t p, int t) {
+  constexpr int U = TPP < 64 ? 1 : 4;
   const float *a = s.logp + p * s.steps, *r = s.ref ? s.ref + p * s.steps : nullptr;
   const uint8_t* m = s.mask ? s.mask + p * s.steps : nullptr;
   const int64_t n = s.steps / 4;
   double v = 0.0;
-#pragma unroll 4
-  for (int64_t q = t; q < n; q += TPP) {
-    Reg<float> x, y;
-    y.w[0] = y.w[1] = y.w[2] = y.w[3] = 0;
-    uint32_t keep = 0xffffffffu;
-    x.load(a + q * 4);
-    if (r) y.load(r + q * 4);
-    if (m) keep = ((const Bytes4*)(m + q * 4))->w;
+  for (int64_t q = t; q < n; q += U * TPP) {
+    Reg<float> x[U], y[U];
+    uint32_t keep[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double d = (double)__uint_as_float(x.w[j]) - (double)__uint_as_float(y.w[j]);
-      v += keep >> 8 * j & 255u ? d : 0.0;
+    for (int u = 0; u < U; ++u) {
+      const int64_t o = q + u * TPP;
+      keep[u] = o < n ? 0xffffffffu : 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[u].w[j] = y[u].w[j] = 0;
+      if (o < n) {
+        x[u].load(a + o * 4);
+        if (r) y[u].load(r + o * 4);
+        if (m) keep[u] = ((const Bytes4*)(m + o * 4))->w;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double d = (double)__uint_as_float(x[u].w[j]) - (double)__uint_as_float(y[u].w[j]);
+        v += keep[u] >> 8 * j & 255u ? d : 0.0;
+      }
   }
   const int64_t j = n * 4 + t;
   if (t < 4 && j < s.steps && (!m || m[j])) v += (double)a[j] - (r ? (double)r[j] : 0.0);
@@ -716,16 +733,16 @@ struct PairIo {
   float *margin, *coef, *loss;
   double* part;
 };
-// TPP threads per pair: a wave where the sequences are short, a block where they are long.
+// TPP threads per pair: 16 lanes or a wave where the sequences are short, a block where they are long.
 template <int TPP> __global__ void __launch_bounds__(256) k_pairs(PairIo io) {
   __shared__ double sd[4];
   const int t = threadIdx.x % TPP;
   double loss = 0.0;
   for (int64_t p = (int64_t)blockIdx.x * (256 / TPP) + threadIdx.x / TPP; p < io.pairs; p += (int64_t)gridDim.x * (256 / TPP)) {
     double h = side_sum<TPP>(io.w, p, t) - side_sum<TPP>(io.l, p, t);
-    h = TPP == 64 ? wave_sum(h) : block_sum<256>(h, sd);
+    h = TPP <= 64 ? wave_sum<TPP <= 64 ? TPP : 64>(h) : block_sum<256>(h, sd);
     if (t == 0) {
-      const double z = io.beta * h, e = exp(-fabs(z)), lp = log1p(e);
+      const double z = io.beta * h, e = exp64(-fabs(z)), lp = log1p(e);
       const double neg = (z < 0.0 ? -z : 0.0) + lp, pos = (z > 0.0 ? z : 0.0) + lp;      // -ln sigmoid(z), -ln sigmoid(-z)
       const double small = e / (1.0 + e), big = 1.0 / (1.0 + e), up = z >= 0.0 ? big : small, down = z >= 0.0 ? small : big;   // sigmoid(z), sigmoid(-z)
       io.margin[p] = (float)z;
@@ -1038,7 +1055,8 @@ extern "C" int ps_policy_loss(const ps_decisions* d, const ps_policy_terms* q, f
   Launches run{(hipStream_t)stream};
   const RowPlan p = r.rows ? plan_rows(r.rows, r.k, d->dtype == PS_F32 ? 4 : 2) : RowPlan{0, 0, 1, 0};
   const RowSpace w(workspace, p, r.rows);
-  const bool counted = r.mask && r.rows > kCountInline;
+  // the valid rows of a short mask are counted by every block for itself (1 - 2 us, all at once where the blocks are few), else by a launch (5 us)
+  const bool counted = r.mask && (r.rows > 16384 || p.grid > 1024);
   io.p = Policy{q->old_logp, q->advantage, q->ref_logp, 1.0 - q->clip_low, 1.0 + q->clip_high, q->kl_coef, q->scale, counted ? w.count : nullptr, q->mean};
   io.logp = logp;
   io.stat = (float2*)stat;
@@ -1073,11 +1091,11 @@ extern "C" int ps_preference_loss(const ps_preference* q, float* loss, float* ma
   const double scale = q->scale / (q->mean ? (double)q->pairs : 1.0);
   const PairIo io{Side{q->better, q->better_ref, q->better_mask, q->better_steps}, Side{q->worse, q->worse_ref, q->worse_mask, q->worse_steps}, q->pairs, q->beta, q->label_smoothing,
                   scale, margin, coef, loss, (double*)workspace};
-  // a wave per pair up to 512 steps of its longer side, a block beyond; 16 such waves' pairs or less are one block's, which then needs no second launch
-  const bool wave = (q->better_steps > q->worse_steps ? q->better_steps : q->worse_steps) <= 512;
-  const int grid = wave ? (q->pairs <= 16 ? 1 : block_grid((q->pairs + 3) / 4)) : block_grid(q->pairs);
-  if (wave) run(k_pairs<64>, grid, 256, io);
-  else run(k_pairs<256>, grid, 256, io);
+  // 16 lanes per pair up to 64 steps of its longer side, a wave up to 512, a block beyond; pairs that fit one block need no second launch
+  const int64_t steps = q->better_steps > q->worse_steps ? q->better_steps : q->worse_steps;
+  const int per_block = steps <= 64 ? 16 : steps <= 512 ? 4 : 1;
+  const int grid = block_grid((q->pairs + per_block - 1) / per_block);
+  run(per_block == 16 ? k_pairs<16> : per_block == 4 ? k_pairs<64> : k_pairs<256>, grid, 256, io);
   if (grid > 1) run(k_pairs_finish, 1, 256, (const double*)workspace, grid, scale, loss);
   return run.result("ps_preference_loss");
 }
