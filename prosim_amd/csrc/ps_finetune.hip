@@ -394,20 +394,39 @@ template <typename T> __device__ __forceinline__ void grad_piece(Reg<T>& v, cons
     for (int i = 0; i < 4; ++i) v.w[i] ^= s.sign;
   }
 }
-// Thread t of TPR owns the piece the chosen column c lies in (pieces of V elements dealt out in turn from column j0, a tail of single elements behind
-// the last whole one): it writes that element once more, whole.
-template <typename T, int TPR> __device__ __forceinline__ void chosen_element(T* dx, int64_t j0, int64_t j1, int64_t c, int t, float xc, float m, float scale, float coef) {
-  if (c < j0 || c >= j1) return;
-  const int64_t o = c - j0, n = (j1 - j0) / Reg<T>::N;
-  const int owner = o < n * Reg<T>::N ? (int)(o / Reg<T>::N % TPR) : (int)(o - n * Reg<T>::N);
-  if (t == owner) dx[c] = from_f32<T>(fmaf(exp_of<T>(xc - m), scale, coef));
+// How TPR threads share a stretch of `len` elements at p: whole 16-byte pieces from the first aligned address on, dealt out in turn, and the elements before
+// and behind them (`edges` of them, a thread each).  Rows of odd length start anywhere; unaligned pieces work on gfx950, but a wave's kilobyte then
+// lies across nine cache lines instead of eight and every lane's 16 bytes across two of the cache's banks' words (3001 x 50021 fp16: 67 us unaligned).
+template <typename T, int TPR> struct Shared {
+  static constexpr int V = Reg<T>::N;
+  static constexpr int ALIGN = TPR >= 128 ? 128 : TPR >= 16 ? TPR : sizeof(T) == 4 ? 16 : (int)sizeof(T);     // bytes; the edges have to fit the threads
+  static_assert(ALIGN / (int)sizeof(T) + V - 2 <= TPR || ALIGN == (int)sizeof(T), "a thread per edge element");
+  int head, pieces, edges;
+  __device__ __forceinline__ Shared(const T* p, int64_t len) {
+    const int lead = (int)(-(uintptr_t)p & (ALIGN - 1)) / (int)sizeof(T);
+    head = lead < len ? lead : (int)len;
+    pieces = (int)((len - head) / V);
+    edges = (int)(len - (int64_t)pieces * V);
+  }
+  // column of thread t's edge element (t < edges)
+  __device__ __forceinline__ int64_t edge(int t) const { return t < head ? t : (int64_t)pieces * V + t; }
+  // the thread that writes column o
+  __device__ __forceinline__ int owner(int64_t o) const {
+    if (o < head) return (int)o;
+    const int64_t q = (o - head) / V;
+    return q < pieces ? (int)(q % TPR) : (int)(o - (int64_t)pieces * V);
+  }
+};
+// The chosen element of a stretch (column o of it, outside for most stretches), written once more and whole by the thread that wrote its piece.
+template <typename T, int TPR> __device__ __forceinline__ void chosen_element(T* dx, const Shared<T, TPR>& sh, int64_t len, int64_t o, int t, float xc, float m, float scale, float coef) {
+  if (o >= 0 && o < len && t == sh.owner(o)) dx[o] = from_f32<T>(fmaf(exp_of<T>(xc - m), scale, coef));
 }
-template <typename T, int THREADS> __device__ __forceinline__ void zero_row(T* dx, int64_t k, int t) {
+template <typename T, int TPR> __device__ __forceinline__ void zero_row(T* dx, int64_t len, int t) {
   Reg<T> z;
   z.w[0] = z.w[1] = z.w[2] = z.w[3] = 0;
-  const int64_t nv = k / Reg<T>::N;
-  for (int64_t q = t; q < nv; q += THREADS) z.store(dx + q * Reg<T>::N);
-  if (nv * Reg<T>::N + t < k && t < Reg<T>::N) dx[nv * Reg<T>::N + t] = from_f32<T>(0.0f);
+  const Shared<T, TPR> sh(dx, len);
+  for (int q = t; q < sh.pieces; q += TPR) z.store(dx + sh.head + (int64_t)q * Reg<T>::N);
+  if (t < sh.edges) dx[sh.edge(t)] = from_f32<T>(0.0f);
 }
 
 // Rows that fit the registers of TPR threads (8 .. 64 lanes of a wave, or that many waves of a block), NV 16-byte pieces per thread: one read of the
@@ -415,7 +434,6 @@ template <typename T, int THREADS> __device__ __forceinline__ void zero_row(T* d
 // constants in registers all the time.
 template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_rows_held(RowIo io) {
   constexpr int THREADS = TPR <= 64 ? 256 : TPR, WAVES = TPR <= 64 ? 1 : TPR / 64, LANES = TPR < 64 ? TPR : 64, V = Reg<T>::N;
-  static_assert(TPR >= V, "the elements behind the last whole piece have a thread each");
   __shared__ double sd[3 * THREADS / 64];
   __shared__ Part joined[WAVES];
   const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
@@ -424,7 +442,7 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
   int64_t count = 0;
   if (MODE == POLICY) weight = weight_of<THREADS>(io, &count, sd);
   const Rows& r = io.r;
-  const int t = threadIdx.x % TPR, nv = (int)(r.k / V), rest = (int)(r.k - (int64_t)nv * V);
+  const int t = threadIdx.x % TPR;
   // (where a wave has one row, its addresses live in scalar registers)
   const int64_t i = block * (THREADS / TPR) + (TPR < 64 ? (int)threadIdx.x / TPR : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR));
   if (i < r.rows) {
@@ -435,12 +453,13 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
     } else {
       const T* x = (const T*)r.x + i * r.stride;
       const int64_t c = choice_of(r, i);        // (the first load: the chosen logit's address waits for nothing else)
+      const Shared<T, TPR> sh(x, r.k);
+      const int nv = sh.pieces;
       Reg<T> v[NV];
 #pragma unroll
       for (int q = 0; q < NV; ++q)
-        if (q * TPR + t < nv) v[q].load_once(x + q * (TPR * V) + (uint32_t)(t * V));
-      const int64_t tail = (int64_t)nv * V + t;
-      const float last = t < rest ? to_f32(x[tail]) : -INFINITY;
+        if (q * TPR + t < nv) v[q].load_once(x + sh.head + q * (TPR * V) + (uint32_t)(t * V));
+      const float last = t < sh.edges ? to_f32(x[sh.edge(t)]) : -INFINITY;
       const bool ok = c >= 0 && c < r.k;
       const float xc = to_f32(x[ok ? c : 0]);
       const RowTerms terms = MODE == POLICY ? terms_of(io.p, i) : RowTerms{};
@@ -484,12 +503,12 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
           if (q * TPR + t < nv) {
             v[q].forget();
             grad_piece<T>(v[q], gs);
-            if (GRAD == GRAD_PAST) v[q].store_once(dx + q * (TPR * V) + (uint32_t)(t * V));
-            else v[q].store(dx + q * (TPR * V) + (uint32_t)(t * V));
+            if (GRAD == GRAD_PAST) v[q].store_once(dx + sh.head + q * (TPR * V) + (uint32_t)(t * V));
+            else v[q].store(dx + sh.head + q * (TPR * V) + (uint32_t)(t * V));
             __builtin_amdgcn_sched_barrier(0);
           }
-        if (t < rest) dx[tail] = from_f32<T>(exp_of<T>(last - a.m) * scale);
-        if (ok) chosen_element<T, TPR>(dx, 0, r.k, c, t, xc, a.m, scale, e.coef);
+        if (t < sh.edges) dx[sh.edge(t)] = from_f32<T>(exp_of<T>(last - a.m) * scale);
+        chosen_element<T, TPR>(dx, sh, r.k, c, t, xc, a.m, scale, e.coef);
       }
     }
   }
@@ -501,18 +520,20 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
 template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(const T* x, int64_t j0, int64_t j1, Part* slots) {
   constexpr int V = Reg<T>::N, U = 4;
   Part a{0.0, -INFINITY};
-  const int64_t n = (j1 - j0) / V;
+  x += j0;
+  const Shared<T, THREADS> sh(x, j1 - j0);
+  const int n = sh.pieces;
   auto raise = [&](float m) {
     if (m > a.m) {
       if (a.s != 0.0) a.s *= (double)exp_of<T>(a.m - m);      // (nothing yet, or -inf alone: 0 stays 0)
       a.m = m;
     }
   };
-  for (int64_t q = threadIdx.x; q < n; q += U * THREADS) {
+  for (int q = threadIdx.x; q < n; q += U * THREADS) {
     Reg<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (q + u * THREADS < n) v[u].load(x + j0 + (q + u * THREADS) * V);
+      if (q + u * THREADS < n) v[u].load(x + sh.head + (int64_t)(q + u * THREADS) * V);
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -535,9 +556,8 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
         a.s += (double)e;
       }
   }
-  const int64_t tail = j0 + n * V + threadIdx.x;
-  if (tail < j1) {
-    const float f = to_f32(x[tail]);
+  if ((int)threadIdx.x < sh.edges) {
+    const float f = to_f32(x[sh.edge(threadIdx.x)]);
     raise(f);
     a.s += (double)exp_of<T>(f - base_of(a.m));
   }
@@ -549,18 +569,21 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
   return join_lanes<THREADS / 64>(a);
 }
 template <typename T, int THREADS> __device__ __forceinline__ void stream_grad(const T* x, T* dx, int64_t j0, int64_t j1, float m, float scale, float coef, int64_t c, float xc) {
-  constexpr int V = Reg<T>::N;
-  const int64_t n = (j1 - j0) / V;
+  x += j0;
+  dx += j0;
+  const Shared<T, THREADS> sh(x, j1 - j0);
   const GradScale gs(m, scale);
-  for (int64_t q = threadIdx.x; q < n; q += THREADS) {
+  for (int q = threadIdx.x; q < sh.pieces; q += THREADS) {
     Reg<T> v;
-    v.load_once(x + j0 + q * V);
+    v.load_once(x + sh.head + (int64_t)q * Reg<T>::N);
     grad_piece<T>(v, gs);
-    v.store(dx + j0 + q * V);
+    v.store(dx + sh.head + (int64_t)q * Reg<T>::N);
   }
-  const int64_t tail = j0 + n * V + threadIdx.x;
-  if (tail < j1) dx[tail] = from_f32<T>(exp_of<T>(to_f32(x[tail]) - m) * scale);
-  chosen_element<T, THREADS>(dx, j0, j1, c, threadIdx.x, xc, m, scale, coef);
+  if ((int)threadIdx.x < sh.edges) {
+    const int64_t j = sh.edge(threadIdx.x);
+    dx[j] = from_f32<T>(exp_of<T>(to_f32(x[j]) - m) * scale);
+  }
+  chosen_element<T, THREADS>(dx, sh, j1 - j0, c - j0, threadIdx.x, xc, m, scale, coef);
 }
 
 // Rows longer than the registers of a block: a pass for the statistics, a second one for the gradient.  One row per block (see k_rows_held).
@@ -646,21 +669,42 @@ template <typename T, int G> __global__ void __launch_bounds__(256) k_grad_short
       dx[i * k + j] = from_f32<T>(coef == 0.0f ? 0.0f : fmaf(exp_of<T>(to_f32(x[j]) - st.x), scale, j == c ? coef : 0.0f));
   }
 }
-// ... longer rows: blocks of `step` elements, splits of them per row.
-template <typename T> __global__ void __launch_bounds__(256) k_grad_long(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, int splits, int64_t step, T* dx) {
+// ... longer rows: stretches of kGradPieces pieces per thread, `splits` of them per row.  A block per stretch -- or, where the call most likely has nothing
+// to do (skip_one), few blocks that would share them: 65536 blocks that only return take 10 us, 1024 take 2.
+// 8192 x 32768 bf16: 8 KB per block 168 us (6.2 TB/s), 4 KB 190, 16 KB 180, 32 KB 195; a loop of single pieces over 16 KB 205.
+constexpr int kGradPieces = 2;
+template <typename T> constexpr int64_t grad_step() { return 256 * kGradPieces * Reg<T>::N; }
+template <typename T> __global__ void __launch_bounds__(256) k_grad_long(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, int splits, T* grad) {
   const float g = gain ? *gain : 1.0f;
   if (skip_one && g == 1.0f) return;
-  for (int64_t b = blockIdx.x; b < r.rows * splits; b += gridDim.x) {
-    const int64_t i = b / splits, j0 = (b - i * splits) * step, j1 = min(j0 + step, r.k);
+  const int t = threadIdx.x;
+  for (int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x; b < r.rows * splits; b += (int64_t)gridDim.x * gridDim.y) {
+    const int64_t i = b / splits, j0 = (b - i * splits) * grad_step<T>();
+    const int64_t len = min(grad_step<T>(), r.k - j0), c = choice_of(r, i) - j0;
+    const float2 st = stat[i];
     const float coef = r.mask && !r.mask[i] ? 0.0f : coef_in[i] * g;
+    T* dx = grad + i * r.k + j0;
     if (coef == 0.0f) {
-      zero_row<T, 256>(dx + i * r.k + j0, j1 - j0, threadIdx.x);
+      zero_row<T, 256>(dx, len, t);
       continue;
     }
-    const float2 st = stat[i];
-    const T* x = (const T*)r.x + i * r.stride;
-    const int64_t c = choice_of(r, i);
-    stream_grad<T, 256>(x, dx + i * r.k, j0, j1, st.x, -coef * st.y, coef, c, to_f32(x[c >= j0 && c < j1 ? c : j0]));
+    const T* x = (const T*)r.x + i * r.stride + j0;
+    const Shared<T, 256> sh(x, len);
+    Reg<T> v[kGradPieces];
+#pragma unroll
+    for (int q = 0; q < kGradPieces; ++q)
+      if (q * 256 + t < sh.pieces) v[q].load_once(x + sh.head + q * (256 * Reg<T>::N) + t * Reg<T>::N);
+    const float last = t < sh.edges ? to_f32(x[sh.edge(t)]) : 0.0f, xc = c >= 0 && c < len ? to_f32(x[c]) : 0.0f;
+    const float scale = -coef * st.y;
+    const GradScale gs(st.x, scale);
+#pragma unroll
+    for (int q = 0; q < kGradPieces; ++q)
+      if (q * 256 + t < sh.pieces) {
+        grad_piece<T>(v[q], gs);
+        v[q].store(dx + sh.head + q * (256 * Reg<T>::N) + t * Reg<T>::N);
+      }
+    if (t < sh.edges) dx[sh.edge(t)] = from_f32<T>(exp_of<T>(last - st.x) * scale);
+    chosen_element<T, 256>(dx, sh, len, c, t, xc, st.x, scale, coef);
   }
 }
 
@@ -800,24 +844,39 @@ struct ClipTable {
   int32_t first[kClipSlots];             // first block of the range
   int n, blocks, block0;                 // block0: index of the launch's first block among the partial sums
 };
-// the elements [a, e) of range s that block b has
-template <typename T> __device__ __forceinline__ T* clip_part(const ClipTable& t, int b, int* len) {
-  int lo = 0, hi = t.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.first[mid] <= b) lo = mid; else hi = mid - 1;
+// the elements block b has of its range: whole pieces from a cache line's start on, and, for the range's first block, those before it
+template <typename T> struct ClipPart {
+  T* g;               // first piece
+  int n, head, rest;  // whole pieces; elements before (at most 127 bytes) and behind them
+  __device__ __forceinline__ ClipPart(const ClipTable& t, int b) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (t.first[mid] <= b) lo = mid; else hi = mid - 1;
+    }
+    T* p = (T*)t.ptr[lo];
+    const int64_t numel = t.numel[lo];
+    int64_t lead = (int64_t)(-(uintptr_t)p & 127) / (int64_t)sizeof(T);
+    if (lead > numel) lead = numel;
+    const int64_t a = lead + (int64_t)(b - t.first[lo]) * clip_chunk<T>(), left = numel - a;
+    const int len = (int)(left < 0 ? 0 : left < clip_chunk<T>() ? left : clip_chunk<T>());
+    g = p + a;
+    n = len / Reg<T>::N;
+    rest = len - n * Reg<T>::N;
+    head = b == t.first[lo] ? (int)lead : 0;
   }
-  const int64_t a = (int64_t)(b - t.first[lo]) * clip_chunk<T>();
-  *len = (int)min(clip_chunk<T>(), (int64_t)t.numel[lo] - a);
-  return (T*)t.ptr[lo] + a;
-}
+  __device__ __forceinline__ T* edge() const {      // this thread's element beside the pieces, or NULL
+    const int t = threadIdx.x;
+    return t < head ? g - head + t : t < head + rest ? g + n * Reg<T>::N + (t - head) : nullptr;
+  }
+};
 // Sum of squares of a block's elements, in 64 bits from the square on (a 32-bit square overflows from 1.8e19 and vanishes below 3.7e-23).
 template <typename T> __global__ void __launch_bounds__(256) k_clip_norm(ClipTable t, double* part) {
   constexpr int V = Reg<T>::N;
   __shared__ double sd[4];
-  int len;
-  const T* g = clip_part<T>(t, blockIdx.x, &len);
-  const int n = len / V;
+  const ClipPart<T> part_of(t, blockIdx.x);
+  const T* g = part_of.g;
+  const int n = part_of.n;
   Reg<T> v[kClipPieces];
 #pragma unroll
   for (int q = 0; q < kClipPieces; ++q) {
@@ -825,8 +884,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_clip_norm(ClipTab
     if (q * 256 + (int)threadIdx.x < n) v[q].load_once(g + q * (256 * V) + threadIdx.x * V);
   }
   double a = 0.0;
-  if (n * V + (int)threadIdx.x < len) {
-    const double d = (double)to_f32(g[n * V + threadIdx.x]);
+  if (const T* e = part_of.edge()) {
+    const double d = (double)to_f32(*e);
     a = d * d;
   }
 #pragma unroll
@@ -853,17 +912,14 @@ template <typename T> __global__ void __launch_bounds__(256) k_clip_scale(ClipTa
   constexpr int V = Reg<T>::N;
   const float c = *coef;
   if (c == 1.0f) return;
-  int len;
-  T* g = clip_part<T>(t, t.blocks - 1 - blockIdx.x, &len);
-  const int n = len / V;
+  const ClipPart<T> part_of(t, t.blocks - 1 - blockIdx.x);
+  T* g = part_of.g;
+  const int n = part_of.n;
   Reg<T> v[kClipPieces];
 #pragma unroll
   for (int q = 0; q < kClipPieces; ++q)
     if (q * 256 + (int)threadIdx.x < n) v[q].load_once(g + q * (256 * V) + threadIdx.x * V);
-  if (n * V + (int)threadIdx.x < len) {
-    T* e = g + n * V + threadIdx.x;
-    *e = from_f32<T>(to_f32(*e) * c);
-  }
+  if (T* e = part_of.edge()) *e = from_f32<T>(to_f32(*e) * c);
 #pragma unroll
   for (int q = 0; q < kClipPieces; ++q)
     if (q * 256 + (int)threadIdx.x < n) {
@@ -892,6 +948,12 @@ struct Launches {
   int result(const char* what) const { return err == hipSuccess ? PS_OK : set_error(PS_E_HIP, "%s: %s", what, hipGetErrorString(err)); }
 };
 int block_grid(int64_t rows) { return (int)(rows < kMaxGrid ? rows : kMaxGrid); }
+
+// more blocks than one dimension takes threads for: lines of 65536 (the kernels drop what the last line has too many)
+dim3 grid2d(int64_t blocks) {
+  const int64_t wide = 1 << 16;
+  return dim3((unsigned)(blocks < wide ? blocks : wide), (unsigned)((blocks + wide - 1) / wide));
+}
 
 int check_rows(const ps_decisions* d, const char* what, Rows* r) {
   if (!d) return set_error(PS_E_ARG, "%s: no decisions", what);
@@ -946,8 +1008,7 @@ RowPlan plan_rows(int64_t rows, int64_t k, int size) {
 }
 template <typename T, int MODE, int GRAD> void launch_rows(Launches& run, const RowIo& io, const RowPlan& p, Part* parts) {
   const int64_t k = io.r.k, pieces = k / Reg<T>::N;
-  const int wide = 1 << 16;
-  const dim3 rows2d(p.grid < wide ? (int)p.grid : wide, (int)((p.grid + wide - 1) / wide));
+  const dim3 rows2d = grid2d(p.grid);
   constexpr int G1 = GRAD == GRAD_PAST ? GRAD_KEPT : GRAD;       // (the kernels that make no difference)
   if (p.kind == 0) {
     if (k <= 4) run(k_rows_short<T, 4, 1, MODE, G1>, (int)p.grid, 256, io);
@@ -1031,10 +1092,9 @@ extern "C" int ps_choice_grad(const ps_decisions* d, const float* coef, const fl
       const int64_t b = (r.rows + 256 / g - 1) / (256 / g);
       run(g == 4 ? k_grad_short<T, 4> : g == 16 ? k_grad_short<T, 16> : k_grad_short<T, 64>, (int)(b < kMaxGrid ? b : kMaxGrid), 256, r, coef, st, gain, skip_if_one, (T*)grad);
     } else {
-      const int64_t step = 256 * Reg<T>::N * 4;         // 16 KB per block and turn
-      const int splits = (int)((r.k + step - 1) / step);
-      const int64_t b = r.rows < kMaxGrid ? r.rows * splits : kMaxGrid;
-      run(k_grad_long<T>, (int)(b < kMaxGrid ? b : kMaxGrid), 256, r, coef, st, gain, skip_if_one, splits, step, (T*)grad);
+      const int splits = (int)((r.k + grad_step<T>() - 1) / grad_step<T>());
+      const int64_t all = r.rows * splits;
+      run(k_grad_long<T>, grid2d(skip_if_one && all > 1024 ? 1024 : all), 256, r, coef, st, gain, skip_if_one, splits, (T*)grad);
     }
     return 0;
   });
