@@ -986,7 +986,10 @@ RowPlan plan_rows(int64_t rows, int64_t k, int size) {
   if (k <= kShort) {
     const int g = k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : 32;
     p.grid = rows <= 2 * 256 / g ? 1 : grid(256 / g, kMaxGrid);      // (two turns of one block cost less than the launch that joins blocks)
-  } else if (rows <= 128 && bytes >= 32768) {
+  } else if (pieces > 8192 && rows <= (pieces > 16384 ? 128 : 64)) {
+    // Several blocks to a row cost a second launch and a second read; they pay where a block alone would be long at it and most of the chip idle.
+    // bf16 policy loss with gradient, one block / split: 131072 elements 1 row 16.8 / 11.3 us, 32 rows 23.9 / 14.6, 64 rows 24.8 / 19.0, 128 rows
+    // 27.6 / 32.2; 32768 elements 1 row 8.6 / 11.2, 64 rows 13.0 / 12.8, 128 rows 13.2 / 14.8.
     p.kind = 3;
     const int64_t want = 512 / rows, most = bytes / 8192;
     p.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);

@@ -168,6 +168,78 @@ def test_policy_loss(ft, rows, k, dtype, masked):
     check_policy(ft, x, c, old, adv, None, mask, 0.0, "sum", 0.25)
 
 
+# every way rows are laid out over threads (groups of 8 .. 64 lanes, 2 .. 16 waves, two passes, split rows), at its borders
+BORDERS = [32, 33, 40, 63, 64, 65, 100, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2048, 2050, 4096, 4103, 8192, 8199, 16390, 32775, 65543]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (0, 1), (5, 3), (64, 0)])
+def test_row_lengths_at_odd_addresses(ft, dtype, pad, offset):
+    """Rows of every length class, beginning at any element, dense or with a gap behind each (then the gradient's rows are aligned otherwise than the logits')."""
+    rows = 70
+    for k in BORDERS:
+        n = rows if k < 20000 else 3
+        flat = (rand(n * (k + pad) + offset, seed=k) * 2).to(dtype).to(dev())
+        x = flat[offset:].view(n, k + pad)[:, :k]
+        c = torch.randint(0, k, (n,), generator=torch.Generator().manual_seed(k)).to(dev())
+        c[0], c[1] = 0, k - 1
+        now = plain_logp(x, c)
+        old = (now + 0.1).float()
+        adv = rand(n, seed=1).to(dev())
+        mask = torch.ones(n, dtype=torch.bool, device=dev())
+        mask[-1] = False
+        check_policy(ft, x, c, old, adv, None, mask, 0.0, "sum", 1.0)
+        leaf = x.detach().requires_grad_(True)
+        out = ft.choice_logp(leaf, c, mask=mask)
+        close(out, torch.where(mask, now, 0.0), U * now.abs() + row_slack(k), f"logp of {k}")
+        g = rand(n, seed=3).to(dev())
+        grad, = torch.autograd.grad(out, leaf, g)
+        g = torch.where(mask, g, 0.0)
+        close(grad, plain_grad(x, c, g), grad_tol(x, c, g, 2 * U * g.double().abs(), dtype), f"gradient of {k}")
+
+
+def test_more_blocks_than_one_grid_dimension(ft):
+    """70001 rows of a block each, and ten stretches of the gradient per row: samples around the ends and the 65536th block."""
+    rows, k = 70001, 9001
+    x = torch.zeros((rows, k), dtype=torch.bfloat16, device=dev())
+    pick = torch.tensor([0, 1, 6553, 6554, 65534, 65535, 65536, 65537, 69999, 70000], device=dev())
+    x[pick] = (rand(len(pick), k, seed=2) * 2).to(torch.bfloat16).to(dev())
+    c = torch.full((rows,), k - 1, dtype=torch.int32, device=dev())
+    leaf = x.requires_grad_(True)
+    out = ft.choice_logp(leaf, c)
+    want = plain_logp(x.detach()[pick], c[pick])
+    close(out.detach()[pick], want, U * want.abs() + row_slack(k), "logp")
+    g, = torch.autograd.grad(out, leaf, torch.ones(rows, device=dev()))
+    one = torch.ones_like(want)
+    close(g[pick], plain_grad(x.detach()[pick], c[pick], one), grad_tol(x.detach()[pick], c[pick], one, one * 0, torch.bfloat16), "gradient")
+    rest = torch.ones(rows, dtype=torch.bool, device=dev())
+    rest[pick] = False
+    assert (out.detach()[rest] - out.detach()[2]).abs().max() == 0 and abs(float(out.detach()[2]) + math.log(k)) < 1e-5
+    same = g[2].clone()
+    for a in range(0, rows, 10000):
+        assert (g[a:a + 10000][rest[a:a + 10000]] == same).all()
+    mask = torch.rand(rows, generator=torch.Generator().manual_seed(1)).to(dev()) < 0.5
+    mask[pick] = True
+    o = ft.policy_loss(leaf, c, out.detach(), one[:1].float(), mask=mask, reduction="mean")
+    assert abs(float(o.loss.detach()) + 1.0) < 1e-5
+    gp, = torch.autograd.grad(o.loss, leaf)
+    coef = -one / float(mask.sum())
+    close(gp[pick], plain_grad(x.detach()[pick], c[pick], coef), grad_tol(x.detach()[pick], c[pick], coef, coef.abs() * (8 * U + row_slack(k)), torch.bfloat16), "policy gradient")
+    assert not gp[~mask][:2000].any()
+
+
+@pytest.mark.parametrize("rows,k", [(1500, 5000), (20000, 40), (300, 700)])
+def test_the_mean_counts_valid_rows_in_every_layout(ft, rows, k):
+    x, c, old, adv, ref = policy_inputs(rows, k, torch.float16, seed=3)
+    mask = torch.rand(rows, generator=torch.Generator().manual_seed(6)).to(dev()) < 0.5
+    check_policy(ft, x, c, old, adv, ref, mask, 0.1, "mean", 1.0)
+    check_policy(ft, x, c, old, adv, ref, mask.to(torch.uint8) * 255 != 0, 0.1, "sum", 1e-4)
+    leaf = x.clone().requires_grad_(True)
+    a = ft.policy_loss(leaf, c, old, adv, mask=mask)
+    b = ft.policy_loss(leaf, c, old, adv, mask=mask.to(torch.uint8) * 200)       # (any byte but 0 is valid)
+    assert torch.equal(a.loss, b.loss) and torch.equal(a.logp, b.logp)
+
+
 def test_mean_loss_of_many_rows_counts_its_mask(ft):
     rows, k = 70001, 6
     x, c, old, adv, ref = policy_inputs(rows, k, torch.float32, seed=3)
@@ -252,7 +324,7 @@ def test_no_valid_row(ft, k):
     x, c, old, adv, ref = policy_inputs(3, k, torch.bfloat16, seed=2)
     leaf = x.fill_(float("nan")).requires_grad_(True)
     o = ft.policy_loss(leaf, c, old, adv, ref_logp=ref, mask=torch.zeros(3, dtype=torch.bool, device=dev()), kl_coef=0.1)
-    assert float(o.loss) == 0.0 and float(o.kl) == 0.0 and float(o.clip_frac) == 0.0
+    assert float(o.loss.detach()) == 0.0 and float(o.kl) == 0.0 and float(o.clip_frac) == 0.0
     assert not torch.autograd.grad(o.loss, leaf)[0].any()
 
 
@@ -469,6 +541,30 @@ def test_refusals(ft):
         z.add_(1.0)
         out.sum().backward()
     assert y is not None
+
+
+def test_calls_from_several_threads(ft):
+    """Four host threads, each on a stream of its own, at once."""
+    from concurrent.futures import ThreadPoolExecutor
+    inputs = [policy_inputs(33, 1500 + 100 * i, torch.float16, seed=i) for i in range(4)]
+    def once(a):
+        x, c, old, adv, ref = a
+        leaf = x.detach().requires_grad_(True)
+        o = ft.policy_loss(leaf, c, old, adv, ref_logp=ref, kl_coef=0.1)
+        g, = torch.autograd.grad(o.loss, leaf)
+        return [o.loss.detach(), o.logp, g, ft.clip_grads_([g.clone(), old.clone()], 0.1)]
+    want = [once(a) for a in inputs]
+    torch.cuda.synchronize()
+    def loop(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [once(inputs[i]) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return got
+    with ThreadPoolExecutor(4) as pool:
+        for i, got in enumerate(pool.map(loop, range(4))):
+            for r in got:
+                for a, b in zip(r, want[i]):
+                    assert torch.equal(a, b)
 
 
 def test_equal_inputs_give_equal_bits_on_any_stream(ft):
