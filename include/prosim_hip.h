@@ -350,7 +350,7 @@ typedef struct ps_decisions {
   const uint8_t* mask;
 } ps_decisions;
 
-/* Bytes of workspace ps_choice_logp and ps_policy_loss want for these rows. */
+/* Bytes of workspace ps_choice_logp and ps_policy_loss want for these rows (only rows, choices and dtype are looked at), or a negative error. */
 int64_t ps_choice_workspace(const ps_decisions* d);
 /* logp [rows] = logits[choice] - ln sum exp logits.  stat [rows][2] (or NULL) = (max, 1 / sum exp(logits - max)), what ps_choice_grad needs. */
 int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* workspace, int64_t workspace_bytes, void* stream);

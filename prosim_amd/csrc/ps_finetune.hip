@@ -1045,7 +1045,7 @@ template <typename T, int MODE, int GRAD> void launch_rows(Launches& run, const 
 
 // count | (loss, kl, clipped) per block | partial results of split rows
 int64_t row_space(const ps_decisions* d) {
-  if (!d || d->rows < 1 || d->choices < 1) return 8;
+  if (d->rows < 1 || d->choices < 1) return 8;
   const RowPlan p = plan_rows(d->rows, d->choices, d->dtype == PS_F32 ? 4 : 2);
   return 8 + 24 * (p.kind == 3 ? d->rows : p.grid) + 16 * (p.kind == 3 ? p.grid : 0);
 }
@@ -1061,7 +1061,7 @@ int check_space(const void* p, int64_t bytes, int64_t need, const char* what) {
 }
 }  // namespace
 
-extern "C" int64_t ps_choice_workspace(const ps_decisions* d) { return row_space(d); }
+extern "C" int64_t ps_choice_workspace(const ps_decisions* d) { return d ? row_space(d) : set_error(PS_E_ARG, "ps_choice_workspace: no decisions"); }
 
 extern "C" int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* workspace, int64_t workspace_bytes, void* stream) {
   RowIo io{};
@@ -1219,6 +1219,7 @@ template <typename F> int64_t clip_tables(int32_t n, void* const* ptr, const int
 }  // namespace
 
 extern "C" int64_t ps_clip_grads_workspace(int32_t n, const int64_t* numel, const int32_t* dtype) {
+  if (n < 0 || (n && (!numel || !dtype))) return set_error(PS_E_ARG, "ps_clip_grads_workspace: NULL table");
   int64_t b = 0;
   for (int32_t i = 0; i < n; ++i) b += clip_blocks(numel[i] > 0 ? numel[i] : 0, dtype[i]);
   return 8 * (b + 1);

@@ -58,7 +58,8 @@ def test_policy_loss_terms(lib, bad):
 def test_workspaces_are_checked(lib):
     t = PsPolicyTerms(FAKE, FAKE, None, 0.2, 0.2, 0.0, 1.0, 1)
     need = lib.ps_choice_workspace(_d())
-    assert need > 0
+    assert need > 0 and lib.ps_choice_workspace(None) == -1 and lib.ps_choice_workspace(_d(rows=0)) > 0
+    assert lib.ps_clip_grads_workspace(1, None, None) == -1 and lib.ps_clip_grads_workspace(0, None, None) == 8
     for ws, size in ((None, need), (FAKE, need - 1), (FAKE + 4, need)):
         assert lib.ps_policy_loss(_d(), t, FAKE, FAKE, FAKE, FAKE, None, None, None, ws, size, None) == -1
         assert lib.ps_choice_logp(_d(), FAKE, None, ws, size, None) == -1
