@@ -373,7 +373,7 @@ template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch
 
 // One 16-byte piece of a row's gradient, -coef e^(x - m) inv; the chosen element's share of coef is added behind it (chosen_element).  16-bit results
 // take the factor into the exponent, |scale| e^d = 2^(d log2 e + log2 |scale|), and its sign afterwards: 6 instead of 8 operations an element beside the
-// exponential, at most (|d| + |log2 scale|) 2^-23 relative, a hundredth of their half step.
+// exponential, at most (|d| + |log2 scale|) 2^-23 relative, a few hundredths of their half step.
 struct GradScale {
   float m, scale, log2_scale;
   uint32_t sign;
@@ -395,8 +395,8 @@ template <typename T> __device__ __forceinline__ void grad_piece(Reg<T>& v, cons
   }
 }
 // How TPR threads share a stretch of `len` elements at p: whole 16-byte pieces from the first aligned address on, dealt out in turn, and the elements before
-// and behind them (`edges` of them, a thread each).  Rows of odd length start anywhere; unaligned pieces work on gfx950, but a wave's kilobyte then
-// lies across nine cache lines instead of eight and every lane's 16 bytes across two of the cache's banks' words (3001 x 50021 fp16: 67 us unaligned).
+// and behind them (`edges` of them, a thread each).  Rows of odd length start anywhere; pieces at element alignment work on gfx950 too, but a wave's
+// kilobyte then lies across nine cache lines instead of eight (3001 x 50021 fp16: 67 us, aligned 54 us).
 template <typename T, int TPR> struct Shared {
   static constexpr int V = Reg<T>::N;
   static constexpr int ALIGN = TPR >= 128 ? 128 : TPR >= 16 ? TPR : sizeof(T) == 4 ? 16 : (int)sizeof(T);     // bytes; the edges have to fit the threads
@@ -533,7 +533,7 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
     Reg<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (q + u * THREADS < n) v[u].load(x + sh.head + (int64_t)(q + u * THREADS) * V);
+      if (q + u * THREADS < n) v[u].load_once(x + sh.head + (int64_t)(q + u * THREADS) * V);
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -586,49 +586,24 @@ template <typename T, int THREADS> __device__ __forceinline__ void stream_grad(c
   chosen_element<T, THREADS>(dx, sh, j1 - j0, c - j0, threadIdx.x, xc, m, scale, coef);
 }
 
-// Rows longer than the registers of a block: a pass for the statistics, a second one for the gradient.  One row per block (see k_rows_held).
-template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(512) k_rows_long(RowIo io) {
-  __shared__ double sd[8];
-  __shared__ Part slots[8];
-  const int64_t i = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  if (i >= io.r.rows) return;      // (the last line of a two-dimensional grid)
-  double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
-  int64_t count = 0;
-  if (MODE == POLICY) weight = weight_of<512>(io, &count, sd);
-  const Rows& r = io.r;
-  T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
-  if (r.mask && !r.mask[i]) {
-    if (threadIdx.x == 0) masked_row(io, i);
-    if (GRAD) zero_row<T, 512>(dx, r.k, threadIdx.x);
-  } else {
-    const T* x = (const T*)r.x + i * r.stride;
-    const int64_t c = choice_of(r, i);
-    const bool ok = c >= 0 && c < r.k;
-    const float xc = to_f32(x[ok ? c : 0]);
-    const RowTerms terms = MODE == POLICY ? terms_of(io.p, i) : RowTerms{};
-    const Part a = stream_part<T, 512>(x, 0, r.k, slots);
-    const RowEnd e = end_row<MODE>(io, i, terms, ok, xc, a, weight, threadIdx.x == 0, acc);
-    if (GRAD) stream_grad<T, 512>(x, dx, 0, r.k, a.m, -e.coef * e.inv, e.coef, c, xc);
-  }
-  if (MODE == POLICY) end_block<512, true>(io, i, acc, count, weight, sd);
-}
-
-// Few long rows: `splits` blocks share a row (at most 64), `step` elements each.  First launch: the blocks' (maximum, sum) ...
+// Rows that no block holds, or few and long: `splits` blocks share a row (at most 64), `step` elements each.  First launch: the blocks' (maximum, sum) ...
 template <typename T> __global__ void __launch_bounds__(256) k_split_part(Rows r, int splits, int64_t step, Part* out) {
   __shared__ Part slots[4];
-  const int64_t i = blockIdx.x / splits, j0 = (blockIdx.x % splits) * step;
-  if (r.mask && !r.mask[i]) return;
+  const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, i = b / splits, j0 = (b - i * splits) * step;
+  if (i >= r.rows || (r.mask && !r.mask[i])) return;
   const Part a = stream_part<T, 256>((const T*)r.x + i * r.stride, j0, min(j0 + step, r.k), slots);
-  if (threadIdx.x == 0) out[blockIdx.x] = a;
+  if (threadIdx.x == 0) out[b] = a;
 }
-// ... second launch: joined by every block for its own stretch of the gradient; the row's first block writes what belongs to the row.
-template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(256) k_split_end(RowIo io, int splits, int64_t step, const Part* parts, int blocks_per_row) {
+// ... second launch: joined, the row's end -- by one block per row, or (GRAD) by every block for its own stretch of the gradient as well.
+template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(256) k_split_end(RowIo io, int splits, int64_t step, const Part* parts) {
   __shared__ double sd[4];
+  const Rows& r = io.r;
+  const int per_row = GRAD ? splits : 1;
+  const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, i = b / per_row, j0 = (b - i * per_row) * step, j1 = min(j0 + step, r.k);
+  if (i >= r.rows) return;
   double acc[3] = {0.0, 0.0, 0.0}, weight = 1.0;
   int64_t count = 0;
   if (MODE == POLICY) weight = weight_of<256>(io, &count, sd);
-  const Rows& r = io.r;
-  const int64_t i = blockIdx.x / blocks_per_row, j0 = (blockIdx.x % blocks_per_row) * step, j1 = min(j0 + step, r.k);
   const bool first = j0 == 0 && threadIdx.x == 0;
   T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
   if (r.mask && !r.mask[i]) {
@@ -647,15 +622,13 @@ template <typename T, int MODE, int GRAD> __global__ void __launch_bounds__(256)
     const RowEnd e = end_row<MODE>(io, i, terms, ok, xc, a, weight, first, acc);
     if (GRAD) stream_grad<T, 256>(x, dx, j0, j1, a.m, -e.coef * e.inv, e.coef, c, xc);
   }
-  if (MODE == POLICY && j0 == 0) {       // (uniform over the block)
-    for (int q = 0; q < 3; ++q)
-      if (threadIdx.x == 0) io.part[i * 3 + q] = acc[q];
-  }
+  if (MODE == POLICY && first)
+    for (int q = 0; q < 3; ++q) io.part[i * 3 + q] = acc[q];
 }
 
 // dx = gain * coef (one-hot - p) from the stored statistics (m, 1 / s).  skip_one: dx already holds the result for gain 1.
-// Rows up to 256 elements: G lanes per row ...
-template <typename T, int G> __global__ void __launch_bounds__(256) k_grad_short(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, T* dx) {
+// Short rows: G lanes per row, as in k_rows_short ...
+template <typename T, int G> __global__ void __launch_bounds__(256) k_grad_short(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, T* grad) {
   const float g = gain ? *gain : 1.0f;
   if (skip_one && g == 1.0f) return;
   const int lane = threadIdx.x & (G - 1), k = (int)r.k;
@@ -665,8 +638,46 @@ template <typename T, int G> __global__ void __launch_bounds__(256) k_grad_short
     const float2 st = stat[i];
     const int64_t c = choice_of(r, i);
     const float scale = -coef * st.y;
-    for (int j = lane; j < k; j += G)
-      dx[i * k + j] = from_f32<T>(coef == 0.0f ? 0.0f : fmaf(exp_of<T>(to_f32(x[j]) - st.x), scale, j == c ? coef : 0.0f));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int j = q * G + lane;
+      if (j < k) grad[i * k + j] = from_f32<T>(coef == 0.0f ? 0.0f : fmaf(exp_of<T>(to_f32(x[j]) - st.x), scale, j == c ? coef : 0.0f));
+    }
+  }
+}
+// ... rows of up to 8 TPR pieces: TPR lanes per row, four pieces in flight ...
+template <typename T, int TPR> __global__ void __launch_bounds__(256) k_grad_rows(Rows r, const float* coef_in, const float2* stat, const float* gain, int skip_one, T* grad) {
+  const float g = gain ? *gain : 1.0f;
+  if (skip_one && g == 1.0f) return;
+  const int t = threadIdx.x % TPR;
+  for (int64_t i = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; i < r.rows; i += (int64_t)gridDim.x * (256 / TPR)) {
+    const int64_t c = choice_of(r, i);
+    const float2 st = stat[i];
+    const float coef = r.mask && !r.mask[i] ? 0.0f : coef_in[i] * g;
+    T* dx = grad + i * r.k;
+    if (coef == 0.0f) {
+      zero_row<T, TPR>(dx, r.k, t);
+      continue;
+    }
+    const T* x = (const T*)r.x + i * r.stride;
+    const Shared<T, TPR> sh(x, r.k);
+    const float last = t < sh.edges ? to_f32(x[sh.edge(t)]) : 0.0f, xc = c >= 0 && c < r.k ? to_f32(x[c]) : 0.0f;
+    const float scale = -coef * st.y;
+    const GradScale gs(st.x, scale);
+    for (int q0 = t; q0 < sh.pieces; q0 += 4 * TPR) {
+      Reg<T> v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (q0 + u * TPR < sh.pieces) v[u].load_once(x + sh.head + (q0 + u * TPR) * Reg<T>::N);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (q0 + u * TPR < sh.pieces) {
+          grad_piece<T>(v[u], gs);
+          v[u].store(dx + sh.head + (q0 + u * TPR) * Reg<T>::N);
+        }
+    }
+    if (t < sh.edges) dx[sh.edge(t)] = from_f32<T>(exp_of<T>(last - st.x) * scale);
+    chosen_element<T, TPR>(dx, sh, r.k, c, t, xc, st.x, scale, coef);
   }
 }
 // ... longer rows: stretches of kGradPieces pieces per thread, `splits` of them per row.  A block per stretch -- or, where the call most likely has nothing
@@ -711,10 +722,15 @@ template <typename T> __global__ void __launch_bounds__(256) k_grad_long(Rows r,
 __global__ void __launch_bounds__(1024) k_count(const uint8_t* mask, int64_t n, int64_t* out) {
   __shared__ double sd[16];
   int64_t c = 0;
-  for (int64_t i = threadIdx.x; i < n / 16; i += 1024) {
-    Reg<uint8_t> q;
-    q.load(mask + i * 16);
-    c += nonzero_bytes(q);
+  for (int64_t i = threadIdx.x; i < n / 16; i += 4 * 1024) {      // (four pieces in flight)
+    Reg<uint8_t> q[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      q[u].w[0] = q[u].w[1] = q[u].w[2] = q[u].w[3] = 0;
+      if (i + u * 1024 < n / 16) q[u].load(mask + (i + u * 1024) * 16);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c += nonzero_bytes(q[u]);
   }
   const int64_t rest = n / 16 * 16 + threadIdx.x;
   if (threadIdx.x < 16 && rest < n) c += mask[rest] != 0;
@@ -962,6 +978,7 @@ int check_rows(const ps_decisions* d, const char* what, Rows* r) {
   if (d->dtype != PS_F32 && d->dtype != PS_BF16 && d->dtype != PS_F16) return set_error(PS_E_ARG, "%s: unknown element type", what);
   if (d->choice_bits != 32 && d->choice_bits != 64) return set_error(PS_E_ARG, "%s: choice_bits must be 32 or 64", what);
   if (d->rows && (!d->logits || !d->choice)) return set_error(PS_E_ARG, "%s: NULL logits or choice", what);
+  if (((uintptr_t)d->logits & (d->dtype == PS_F32 ? 3 : 1)) || ((uintptr_t)d->choice & (d->choice_bits / 8 - 1))) return set_error(PS_E_ARG, "%s: logits or choice are not aligned to their elements", what);
   *r = Rows{d->logits, d->rows, d->choices, d->row_stride, d->choice, d->mask, d->choice_bits == 64};
   return PS_OK;
 }
@@ -971,89 +988,113 @@ template <typename F> int by_type(int dtype, F f) {
 }
 
 // How rows are laid out over the chip: a rule on their number, length and type.
+enum RowKind { SHORT, HELD, SPLIT, VERY_LONG };
 struct RowPlan {
-  int kind;             // 0 short, 1 held in registers, 2 long, 3 split
-  int64_t grid;         // blocks
+  RowKind kind;
+  int64_t grid;         // blocks of the first launch
   int splits;
   int64_t step;
+  int64_t parts(int64_t rows) const { return kind == SPLIT || kind == VERY_LONG ? rows : grid; }      // partial sums of the loss
 };
 constexpr int64_t kPastCaches = 256 << 20;      // bytes of the last-level cache
 constexpr int kShort = 32;             // elements a row of k_rows_short may have
+// lanes of a short row, four elements each: the fewest, because a wave pays the end of a row once for all the rows it has
+// (10^6 rows of 6 fp32 with gradient: 8 lanes of one element 69 us, 2 of four 26; of 30 bf16, forward: 32 of one 140 us, 8 of four 41)
+int short_lanes(int64_t k) { return k <= 4 ? 1 : k <= 8 ? 2 : k <= 16 ? 4 : 8; }
 RowPlan plan_rows(int64_t rows, int64_t k, int size) {
   const int64_t bytes = k * size, pieces = k * size / 16;
-  RowPlan p{0, 1, 1, k};
+  RowPlan p{SHORT, 1, 1, k};
   auto grid = [&](int64_t per_block, int64_t most) { const int64_t b = (rows + per_block - 1) / per_block; return b < most ? b : most; };
-  if (k <= kShort) {
-    const int g = k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : 32;
-    p.grid = rows <= 2 * 256 / g ? 1 : grid(256 / g, kMaxGrid);      // (two turns of one block cost less than the launch that joins blocks)
-  } else if (pieces > 8192 && rows <= (pieces > 16384 ? 128 : 64)) {
-    // Several blocks to a row cost a second launch and a second read; they pay where a block alone would be long at it and most of the chip idle.
-    // bf16 policy loss with gradient, one block / split: 131072 elements 1 row 16.8 / 11.3 us, 32 rows 23.9 / 14.6, 64 rows 24.8 / 19.0, 128 rows
-    // 27.6 / 32.2; 32768 elements 1 row 8.6 / 11.2, 64 rows 13.0 / 12.8, 128 rows 13.2 / 14.8.
-    p.kind = 3;
-    const int64_t want = 512 / rows, most = bytes / 8192;
+  auto split = [&](int64_t want) {
     p.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
-    if (p.splits > most) p.splits = (int)most;
     p.step = ((k + p.splits - 1) / p.splits + 63) / 64 * 64;
     p.splits = (int)((k + p.step - 1) / p.step);
     p.grid = rows * p.splits;
+  };
+  if (k <= kShort) {
+    const int g = short_lanes(k);
+    p.grid = rows <= 2 * 256 / g ? 1 : grid(256 / g, kMaxGrid);      // (two turns of one block cost less than the launch that joins blocks)
+  } else if (pieces > 8192 && rows <= 64) {
+    // Several blocks to a row cost a second launch and a second read; they pay where a block alone would be long at it and most of the chip idle.
+    // bf16 policy loss with gradient, one block / split: 131072 elements 1 row 16.8 / 11.3 us, 32 rows 23.9 / 14.6, 64 rows 24.8 / 19.0, 128 rows
+    // 27.6 / 32.2; 32768 elements 1 row 8.6 / 11.2, 64 rows 13.0 / 12.8, 128 rows 13.2 / 14.8.
+    p.kind = SPLIT;
+    split(512 / rows);
   } else if (pieces <= 512) {
-    p.kind = 1;
+    p.kind = HELD;
     p.grid = grid(pieces <= 64 ? 32 : pieces <= 128 ? 16 : pieces <= 256 ? 8 : 4, rows);
   } else if (pieces <= 16384) {
-    p.kind = 1;
+    p.kind = HELD;
     p.grid = rows;
   } else {
-    p.kind = 2;
-    p.grid = rows;
+    p.kind = VERY_LONG;      // (300 x 250000 fp32 with gradient: 162 us; a block per row in two passes 222)
+    split((bytes + 65535) / 65536);
   }
   return p;
 }
+template <typename T> void launch_grad(Launches& run, const Rows& r, const float* coef, const float2* stat, const float* gain, int skip, T* grad) {
+  const int64_t pieces = r.k / Reg<T>::N;
+  auto grid = [&](int lanes) { const int64_t b = (r.rows + 256 / lanes - 1) / (256 / lanes), most = skip ? 512 : 1 << 20; return (int)(b < most ? b : most); };
+  if (r.k <= kShort) {
+    const int g = short_lanes(r.k);
+    run(g == 1 ? k_grad_short<T, 1> : g == 2 ? k_grad_short<T, 2> : g == 4 ? k_grad_short<T, 4> : k_grad_short<T, 8>, grid(g), 256, r, coef, stat, gain, skip, grad);
+  } else if (pieces <= 256) {
+    const int lanes = pieces <= 64 ? 8 : 32;
+    run(lanes == 8 ? k_grad_rows<T, 8> : k_grad_rows<T, 32>, grid(lanes), 256, r, coef, stat, gain, skip, grad);
+  } else {
+    const int splits = (int)((r.k + grad_step<T>() - 1) / grad_step<T>());
+    const int64_t all = r.rows * splits;
+    run(k_grad_long<T>, grid2d(skip && all > 1024 ? 1024 : all), 256, r, coef, stat, gain, skip, splits, grad);
+  }
+}
 template <typename T, int MODE, int GRAD> void launch_rows(Launches& run, const RowIo& io, const RowPlan& p, Part* parts) {
   const int64_t k = io.r.k, pieces = k / Reg<T>::N;
-  const dim3 rows2d = grid2d(p.grid);
+  const dim3 grid = grid2d(p.grid);
   constexpr int G1 = GRAD == GRAD_PAST ? GRAD_KEPT : GRAD;       // (the kernels that make no difference)
-  if (p.kind == 0) {
-    if (k <= 4) run(k_rows_short<T, 4, 1, MODE, G1>, (int)p.grid, 256, io);
-    else if (k <= 8) run(k_rows_short<T, 8, 1, MODE, G1>, (int)p.grid, 256, io);
-    else if (k <= 16) run(k_rows_short<T, 16, 1, MODE, G1>, (int)p.grid, 256, io);
-    else run(k_rows_short<T, 32, 1, MODE, G1>, (int)p.grid, 256, io);
-  } else if (p.kind == 1) {
+  if (p.kind == SHORT) {
+    const int g = short_lanes(k);
+    run(g == 1 ? k_rows_short<T, 1, 4, MODE, G1> : g == 2 ? k_rows_short<T, 2, 4, MODE, G1> : g == 4 ? k_rows_short<T, 4, 4, MODE, G1> : k_rows_short<T, 8, 4, MODE, G1>, grid, 256, io);
+  } else if (p.kind == HELD) {
     // Threads per row by its pieces.  Few threads with many pieces each beat many with few: the end of a row (64-bit functions, reductions) costs
     // every wave of it the same (8192-element rows: 1 x 512 rows of 64 threads x 16 pieces 87 us, 2 x 8 89 us, 4 x 4 114 us), and rows that need not
     // wait for each other overlap one's reading with another's writing (65536-element rows with gradient: 8 waves x 16 pieces 192 us, 16 x 8 251 us).
     constexpr bool fwd = MODE == LOGP;       // (the policy loss takes the same kernel with and without its gradient: the same bits)
-    if (pieces <= 16) run(k_rows_held<T, 8, 2, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 32) run(k_rows_held<T, 8, 4, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 64) run(k_rows_held<T, 8, 8, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 128) run(k_rows_held<T, 16, 8, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 256) run(k_rows_held<T, 32, 8, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 512) run(k_rows_held<T, 64, 8, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 1024) run(k_rows_held<T, 128, 8, MODE, GRAD>, rows2d, 128, io);
-    else if (pieces <= 2048) run(k_rows_held<T, fwd ? 128 : 256, fwd ? 16 : 8, MODE, GRAD>, rows2d, fwd ? 128 : 256, io);
-    else if (pieces <= 4096) run(k_rows_held<T, 256, 16, MODE, GRAD>, rows2d, 256, io);
-    else if (pieces <= 8192) run(k_rows_held<T, 512, 16, MODE, GRAD>, rows2d, 512, io);
-    else run(k_rows_held<T, 1024, 16, MODE, GRAD>, rows2d, 1024, io);
-  } else if (p.kind == 2) {
-    run(k_rows_long<T, MODE, G1>, rows2d, 512, io);
+    if (pieces <= 16) run(k_rows_held<T, 8, 2, MODE, GRAD>, grid, 256, io);
+    else if (pieces <= 32) run(k_rows_held<T, 8, 4, MODE, GRAD>, grid, 256, io);
+    else if (pieces <= 64) run(k_rows_held<T, 8, 8, MODE, GRAD>, grid, 256, io);
+    else if (pieces <= 128) run(k_rows_held<T, 16, 8, MODE, GRAD>, grid, 256, io);
+    else if (pieces <= 256) run(k_rows_held<T, 32, 8, MODE, GRAD>, grid, 256, io);
+    else if (pieces <= 512) run(k_rows_held<T, 64, 8, MODE, GRAD>, grid, 256, io);
+    else if (pieces <= 1024) run(k_rows_held<T, 128, 8, MODE, GRAD>, grid, 128, io);
+    else if (pieces <= 2048) run(k_rows_held<T, fwd ? 128 : 256, fwd ? 16 : 8, MODE, GRAD>, grid, fwd ? 128 : 256, io);
+    else if (pieces <= 4096) run(k_rows_held<T, 256, 16, MODE, GRAD>, grid, 256, io);
+    else if (pieces <= 8192) run(k_rows_held<T, 512, 16, MODE, GRAD>, grid, 512, io);
+    else run(k_rows_held<T, 1024, 16, MODE, GRAD>, grid, 1024, io);
   } else {
-    run(k_split_part<T>, (int)p.grid, 256, io.r, p.splits, p.step, parts);
-    const int per_row = GRAD ? p.splits : 1;
-    run(k_split_end<T, MODE, G1>, (int)(io.r.rows * per_row), 256, io, p.splits, p.step, (const Part*)parts, per_row);
+    run(k_split_part<T>, grid, 256, io.r, p.splits, p.step, parts);
+    if (p.kind == SPLIT) {
+      run(k_split_end<T, MODE, G1>, GRAD ? grid : grid2d(io.r.rows), 256, io, p.splits, p.step, (const Part*)parts);
+    } else {
+      run(k_split_end<T, MODE, GRAD_NONE>, grid2d(io.r.rows), 256, io, p.splits, p.step, (const Part*)parts);
+      if (GRAD) launch_grad<T>(run, io.r, io.coef, io.stat, nullptr, 0, (T*)io.dx);
+    }
   }
 }
 
-// count | (loss, kl, clipped) per block | partial results of split rows
+// count | (loss, kl, clipped) per block | partial results of split rows | (maximum, 1 / sum) and coefficient of very long rows
 int64_t row_space(const ps_decisions* d) {
   if (d->rows < 1 || d->choices < 1) return 8;
   const RowPlan p = plan_rows(d->rows, d->choices, d->dtype == PS_F32 ? 4 : 2);
-  return 8 + 24 * (p.kind == 3 ? d->rows : p.grid) + 16 * (p.kind == 3 ? p.grid : 0);
+  return 8 + 24 * p.parts(d->rows) + (p.kind == SPLIT || p.kind == VERY_LONG ? 16 * p.grid : 0) + (p.kind == VERY_LONG ? 12 * d->rows : 0);
 }
 struct RowSpace {
   int64_t* count;
   double* part;
   Part* parts;
-  RowSpace(void* p, const RowPlan& plan, int64_t rows) : count((int64_t*)p), part((double*)p + 1), parts((Part*)((double*)p + 1 + 3 * (plan.kind == 3 ? rows : plan.grid))) {}
+  float2* stat;
+  float* coef;
+  RowSpace(void* p, const RowPlan& plan, int64_t rows)
+      : count((int64_t*)p), part((double*)p + 1), parts((Part*)(part + 3 * plan.parts(rows))), stat((float2*)(parts + (plan.kind == VERY_LONG ? plan.grid : 0))), coef((float*)(stat + rows)) {}
 };
 int check_space(const void* p, int64_t bytes, int64_t need, const char* what) {
   if (!p || bytes < need || ((uintptr_t)p & 7)) return set_error(PS_E_ARG, "%s: workspace missing, unaligned or smaller than %lld bytes", what, (long long)need);
@@ -1067,7 +1108,7 @@ extern "C" int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, v
   RowIo io{};
   if (int e = check_rows(d, "ps_choice_logp", &io.r)) return e;
   if (!io.r.rows) return PS_OK;
-  if (!logp) return set_error(PS_E_ARG, "ps_choice_logp: NULL logp");
+  if (!logp || ((uintptr_t)stat & 7)) return set_error(PS_E_ARG, "ps_choice_logp: NULL logp, or stat is not aligned");
   if (int e = check_space(workspace, workspace_bytes, row_space(d), "ps_choice_logp")) return e;
   Launches run{(hipStream_t)stream};
   io.logp = logp;
@@ -1086,19 +1127,11 @@ extern "C" int ps_choice_grad(const ps_decisions* d, const float* coef, const fl
   if (int e = check_rows(d, "ps_choice_grad", &r)) return e;
   if (!r.rows) return PS_OK;
   if (!coef || !stat || !grad) return set_error(PS_E_ARG, "ps_choice_grad: NULL coef, stat or grad");
+  if (((uintptr_t)grad & (d->dtype == PS_F32 ? 3 : 1)) || ((uintptr_t)stat & 7)) return set_error(PS_E_ARG, "ps_choice_grad: grad or stat is not aligned");
   Launches run{(hipStream_t)stream};
   by_type(d->dtype, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
-    const float2* st = (const float2*)stat;
-    if (r.k <= 256) {
-      const int g = r.k <= 4 ? 4 : r.k <= 16 ? 16 : 64;
-      const int64_t b = (r.rows + 256 / g - 1) / (256 / g);
-      run(g == 4 ? k_grad_short<T, 4> : g == 16 ? k_grad_short<T, 16> : k_grad_short<T, 64>, (int)(b < kMaxGrid ? b : kMaxGrid), 256, r, coef, st, gain, skip_if_one, (T*)grad);
-    } else {
-      const int splits = (int)((r.k + grad_step<T>() - 1) / grad_step<T>());
-      const int64_t all = r.rows * splits;
-      run(k_grad_long<T>, grid2d(skip_if_one && all > 1024 ? 1024 : all), 256, r, coef, st, gain, skip_if_one, splits, (T*)grad);
-    }
+    launch_grad<T>(run, r, coef, (const float2*)stat, gain, skip_if_one, (T*)grad);
     return 0;
   });
   return run.result("ps_choice_grad");
@@ -1114,16 +1147,17 @@ extern "C" int ps_policy_loss(const ps_decisions* d, const ps_policy_terms* q, f
   if (!(q->kl_coef >= 0.0) || std::isinf(q->kl_coef)) return set_error(PS_E_ARG, "ps_policy_loss: kl_coef must be >= 0 and finite");
   if (!std::isfinite(q->scale)) return set_error(PS_E_ARG, "ps_policy_loss: scale must be finite");
   if (q->kl_coef > 0.0 && !q->ref_logp && r.rows) return set_error(PS_E_ARG, "ps_policy_loss: kl_coef without ref_logp");
+  if (((uintptr_t)grad & (d->dtype == PS_F32 ? 3 : 1)) || ((uintptr_t)stat & 7)) return set_error(PS_E_ARG, "ps_policy_loss: grad or stat is not aligned");
   if (int e = check_space(workspace, workspace_bytes, row_space(d), "ps_policy_loss")) return e;
   Launches run{(hipStream_t)stream};
-  const RowPlan p = r.rows ? plan_rows(r.rows, r.k, d->dtype == PS_F32 ? 4 : 2) : RowPlan{0, 0, 1, 0};
+  const RowPlan p = r.rows ? plan_rows(r.rows, r.k, d->dtype == PS_F32 ? 4 : 2) : RowPlan{SHORT, 0, 1, 0};
   const RowSpace w(workspace, p, r.rows);
   // the valid rows of a short mask are counted by every block for itself (1 - 2 us, all at once where the blocks are few), else by a launch (5 us)
   const bool counted = r.mask && (r.rows > 16384 || p.grid > 1024);
   io.p = Policy{q->old_logp, q->advantage, q->ref_logp, 1.0 - q->clip_low, 1.0 + q->clip_high, q->kl_coef, q->scale, counted ? w.count : nullptr, q->mean};
   io.logp = logp;
-  io.stat = (float2*)stat;
-  io.coef = coef;
+  io.stat = stat || p.kind != VERY_LONG || !grad ? (float2*)stat : w.stat;
+  io.coef = coef || p.kind != VERY_LONG || !grad ? coef : w.coef;
   io.dx = grad;
   io.part = w.part;
   io.loss = loss;
@@ -1134,12 +1168,12 @@ extern "C" int ps_policy_loss(const ps_decisions* d, const ps_policy_terms* q, f
   if (r.rows)
     by_type(d->dtype, [&](auto* t) {
       typedef std::remove_pointer_t<decltype(t)> T;
-      if (grad && past && p.kind == 1) launch_rows<T, POLICY, GRAD_PAST>(run, io, p, w.parts);
+      if (grad && past && p.kind == HELD) launch_rows<T, POLICY, GRAD_PAST>(run, io, p, w.parts);
       else if (grad) launch_rows<T, POLICY, GRAD_KEPT>(run, io, p, w.parts);
       else launch_rows<T, POLICY, GRAD_NONE>(run, io, p, w.parts);
       return 0;
     });
-  if (p.grid != 1 || p.kind == 3) run(k_policy_finish, 1, 256, io, p.kind == 3 ? r.rows : p.grid);      // (a launch of one block has written the results itself)
+  if (p.grid != 1 || p.kind == SPLIT || p.kind == VERY_LONG) run(k_policy_finish, 1, 256, io, p.parts(r.rows));      // (a launch of one block has written the results itself)
   return run.result("ps_policy_loss");
 }
 

@@ -61,8 +61,9 @@ def policy_loss(logits: torch.Tensor, choice: torch.Tensor, old_logp: torch.Tens
     ``advantage``, ``ref_logp`` float32 of the rows' shape (``advantage`` may broadcast to it: one score per rollout), constants.  ``clip_high`` defaults to
     ``clip_low``; ``ref_logp`` is needed when ``kl_coef`` > 0 and only reported as ``kl`` otherwise.  Without a valid row the loss is 0.
 
-    Put the factor of an accumulated or scaled step into ``scale`` rather than multiplying the loss: the forward pass has already written the gradient,
-    and a backward pass that arrives with 1 costs nothing more."""
+    Put the factor of an accumulated or scaled step into ``scale`` rather than multiplying the loss: the forward pass has already written the gradient
+    (a buffer of the logits' size lives from it to the backward pass), and a backward pass that arrives with 1 costs nothing more; any other factor is
+    right too, and costs another pass over the logits."""
     return PolicyLoss(*_finetune.policy_loss(logits, choice, old_logp, advantage, ref_logp, mask, clip_low, clip_high, kl_coef, reduction, scale))
 
 

@@ -25,7 +25,7 @@ def _d(**kw):
 
 
 @pytest.mark.parametrize("bad", [dict(rows=-1), dict(choices=0), dict(choices=1 << 31), dict(row_stride=7), dict(dtype=3), dict(dtype=-1), dict(choice_bits=16),
-                                 dict(logits=None), dict(choice=None)])
+                                 dict(logits=None), dict(choice=None), dict(logits=FAKE + 2), dict(dtype=1, logits=FAKE + 1), dict(choice=FAKE + 4)])
 def test_c_entries_refuse_bad_decisions(lib, bad):
     d = _d(**bad)
     assert lib.ps_choice_logp(d, FAKE, None, FAKE, 1 << 20, None) == -1
@@ -41,6 +41,9 @@ def test_c_entries_refuse_missing_buffers(lib):
     assert lib.ps_choice_logp(_d(), None, None, FAKE, 1 << 20, None) == -1
     for args in ((None, FAKE, FAKE), (FAKE, None, FAKE), (FAKE, FAKE, None)):
         assert lib.ps_choice_grad(_d(), args[0], args[1], None, 0, args[2], None) == -1
+    for d in (_d(), _d(dtype=2)):
+        assert lib.ps_choice_grad(d, FAKE, FAKE, None, 0, FAKE + 1, None) == -1 and lib.ps_choice_grad(d, FAKE, FAKE + 4, None, 0, FAKE, None) == -1
+    assert lib.ps_choice_logp(_d(), FAKE, FAKE + 4, FAKE, 1 << 20, None) == -1
     assert lib.ps_choice_logp(_d(rows=0, logits=None, choice=None), None, None, None, 0, None) == 0     # (no rows: nothing to do)
 
 

@@ -72,7 +72,7 @@ def close(got, want, tol, what=""):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() - tol)[bad].max())} beyond its bound"
 
 
-ROWS_CHOICES = [(1, 1), (5, 1), (1, 2), (3, 3), (1025, 3), (17, 7), (64, 16), (65, 17), (31, 64), (33, 65), (9, 127), (10, 128), (7, 255), (5, 257), (130, 511), (4, 513),
+ROWS_CHOICES = [(40000, 30), (30000, 4), (257, 5), (9000, 8), (1000, 9), (7000, 16), (70, 250), (90, 600), (60, 2048), (1, 1), (5, 1), (1, 2), (3, 3), (1025, 3), (17, 7), (64, 16), (65, 17), (31, 64), (33, 65), (9, 127), (10, 128), (7, 255), (5, 257), (130, 511), (4, 513),
                 (3, 1000), (6, 1024), (5, 2049), (2, 4096), (3, 4099), (2, 8191), (3, 16387), (2, 32768), (1, 50021), (2, 65537), (1, 131072), (2, 131071), (1, 200003),
                 (300, 1111), (2500, 40), (70, 9001)]
 
@@ -198,6 +198,28 @@ def test_row_lengths_at_odd_addresses(ft, dtype, pad, offset):
         close(grad, plain_grad(x, c, g), grad_tol(x, c, g, 2 * U * g.double().abs(), dtype), f"gradient of {k}")
 
 
+@pytest.mark.parametrize("dtype,k", [(torch.float32, 66001), (torch.bfloat16, 140003), (torch.float16, 131080)])
+def test_rows_no_block_can_hold(ft, dtype, k):
+    """More than 64 rows longer than 256 KB: statistics by parts, the end of a row, the gradient, a launch each -- from C also without the caller's statistics."""
+    from prosim_amd.engine import PsDecisions, PsPolicyTerms, load_library
+    rows = 67
+    x, c, old, adv, ref = policy_inputs(rows, k, dtype, seed=12)
+    mask = torch.rand(rows, generator=torch.Generator().manual_seed(6)).to(dev()) < 0.7
+    check_policy(ft, x, c, old, adv, ref, mask, 0.1, "mean", 1.0)
+    leaf = x.detach().requires_grad_(True)
+    o = ft.policy_loss(leaf, c, old, adv, ref_logp=ref, mask=mask, kl_coef=0.1)
+    want, = torch.autograd.grad(o.loss, leaf)
+    lib = load_library()
+    d = PsDecisions(x.data_ptr(), rows, k, k, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], 64, c.data_ptr(), mask.data_ptr())
+    q = PsPolicyTerms(old.data_ptr(), adv.data_ptr(), ref.data_ptr(), 0.2, 0.2, 0.1, 1.0, 1)
+    nums, logp, grad = torch.empty(3, device=dev()), torch.empty(rows, device=dev()), torch.empty_like(x)
+    space = torch.empty(lib.ps_choice_workspace(d), dtype=torch.uint8, device=dev())
+    at = nums.data_ptr()
+    rc = lib.ps_policy_loss(d, q, at, at + 4, at + 8, logp.data_ptr(), None, None, grad.data_ptr(), space.data_ptr(), space.numel(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert torch.equal(grad, want) and torch.equal(logp, o.logp) and torch.equal(nums[0], o.loss.detach()) and torch.equal(nums[1], o.kl)
+
+
 def test_more_blocks_than_one_grid_dimension(ft):
     """70001 rows of a block each, and ten stretches of the gradient per row: samples around the ends and the 65536th block."""
     rows, k = 70001, 9001
@@ -228,7 +250,7 @@ def test_more_blocks_than_one_grid_dimension(ft):
     assert not gp[~mask][:2000].any()
 
 
-@pytest.mark.parametrize("rows,k", [(1500, 5000), (20000, 40), (300, 700)])
+@pytest.mark.parametrize("rows,k", [(1500, 5000), (20000, 40), (300, 700), (40000, 3), (30000, 30), (513, 4), (512, 4), (511, 5)])
 def test_the_mean_counts_valid_rows_in_every_layout(ft, rows, k):
     x, c, old, adv, ref = policy_inputs(rows, k, torch.float16, seed=3)
     mask = torch.rand(rows, generator=torch.Generator().manual_seed(6)).to(dev()) < 0.5
