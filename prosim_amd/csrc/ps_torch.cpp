@@ -39,7 +39,7 @@ int dtype_of(const Tensor& t) {
     default: return -1;
   }
 }
-Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type = at::kFloat) { return at::empty(sizes, like.options().dtype(type)); }
+Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type = at::kFloat) { return at::empty(sizes, at::TensorOptions().device(like.device()).dtype(type)); }
 template <typename T> T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -50,15 +50,14 @@ void check(int rc) {
 }
 
 // A float32 constant of the rows' shape as dense memory.
-Tensor constant(const Tensor& given, const char* name, at::IntArrayRef shape, const Tensor& like, bool broadcast = false) {
-  const Tensor t = given.requires_grad() ? given.detach() : given;       // (a layout copy is no part of the graph)
+Tensor constant(const Tensor& t, const char* name, at::IntArrayRef shape, const Tensor& like, bool broadcast = false) {
   check_gpu(t, name, like);
   TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, name, ": expected float32, got ", type_name(t));
-  if (t.sizes() != shape) {
-    TORCH_CHECK_VALUE(broadcast && at::is_expandable_to(t.sizes(), shape), name, ": expected shape ", shape, ", got ", t.sizes());
-    return t.expand(shape).contiguous();
-  }
-  return t.contiguous();
+  const bool same = t.sizes() == shape;
+  TORCH_CHECK_VALUE(same || (broadcast && at::is_expandable_to(t.sizes(), shape)), name, ": expected shape ", shape, ", got ", t.sizes());
+  if (same && t.is_contiguous()) return t;
+  const at::NoGradGuard quiet;      // (a layout copy is no part of the graph)
+  return t.expand(shape).contiguous();
 }
 Tensor mask_of(const Maybe& m, const char* name, at::IntArrayRef shape, const Tensor& like) {
   if (!m) return Tensor();
@@ -141,7 +140,7 @@ struct Space {
 Tensor choice_grad(const Tensor& logits, const Tensor& choice, const Tensor& mask, const float* stat, const float* coef, const float* gain, Tensor done) {
   const Decisions r(logits, choice, mask);
   const bool ready = done.defined();
-  Tensor grad = ready ? std::move(done) : at::empty(logits.sizes(), logits.options());
+  Tensor grad = ready ? std::move(done) : empty(logits.sizes(), logits, logits.scalar_type());
   check(ps_choice_grad(&r.d, coef, stat, gain, ready, grad.data_ptr(), stream_of(logits)));
   return grad;
 }
@@ -192,7 +191,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Rest& rest, const ps_policy_terms& terms) {
     const Decisions r(logits, rest.choice, rest.mask);
     const Space space(r, true);
-    const Tensor grad = at::empty(logits.sizes(), logits.options());
+    const Tensor grad = empty(logits.sizes(), logits, logits.scalar_type());
     variable_list out = policy_forward(r, terms, space, grad);
     ctx->saved_data["ready"] = grad;
     ctx->save_for_backward({logits, rest.choice, rest.mask, space.all});
@@ -243,8 +242,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     float* coef = (float*)((char*)space.data_ptr() + bytes);
     check(ps_preference_loss(&q, ptr<float>(loss), ptr<float>(margin), coef, space.data_ptr(), bytes, stream_of(better)));
     ctx->save_for_backward({space, b.mask, w.mask});
-    ctx->saved_data["better"] = better.sizes();
-    ctx->saved_data["worse"] = worse.sizes();
+    ctx->saved_data["shapes"] = std::vector<int64_t>{q.pairs, better.dim() == 2 ? q.better_steps : -1, worse.dim() == 2 ? q.worse_steps : -1};      // (-1: [pairs])
     ctx->mark_non_differentiable({margin});
     ctx->set_materialize_grads(false);
     return {loss, margin};
@@ -252,17 +250,17 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
-    const std::vector<int64_t> shape[2] = {ctx->saved_data["better"].toIntVector(), ctx->saved_data["worse"].toIntVector()};
-    const int64_t pairs = shape[0][0];
+    const std::vector<int64_t> shapes = ctx->saved_data["shapes"].toIntVector();
+    const int64_t pairs = shapes[0];
     Tensor out[2];
     for (int i = 0; i < 2; ++i)
-      if (ctx->needs_input_grad(i)) out[i] = empty(shape[i], s[0]);
+      if (ctx->needs_input_grad(i)) out[i] = shapes[1 + i] < 0 ? empty({pairs}, s[0]) : empty({pairs, shapes[1 + i]}, s[0]);
     ps_preference q{};
     q.better_mask = ptr<uint8_t>(s[1]);
     q.worse_mask = ptr<uint8_t>(s[2]);
     q.pairs = pairs;
-    q.better_steps = shape[0].size() == 2 ? shape[0][1] : 1;
-    q.worse_steps = shape[1].size() == 2 ? shape[1][1] : 1;
+    q.better_steps = shapes[1] < 0 ? 1 : shapes[1];
+    q.worse_steps = shapes[2] < 0 ? 1 : shapes[2];
     const Tensor gain = grads[0].contiguous();
     check(ps_preference_grad(&q, (float*)((char*)s[0].data_ptr() + s[0].numel() - 4 * pairs), ptr<float>(gain), ptr<float>(out[0]), ptr<float>(out[1]), stream_of(s[0])));
     return once({out[0], out[1], Tensor(), Tensor(), Tensor()});

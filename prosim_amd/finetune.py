@@ -64,7 +64,7 @@ def policy_loss(logits: torch.Tensor, choice: torch.Tensor, old_logp: torch.Tens
     Put the factor of an accumulated or scaled step into ``scale`` rather than multiplying the loss: the forward pass has already written the gradient
     (a buffer of the logits' size lives from it to the backward pass), and a backward pass that arrives with 1 costs nothing more; any other factor is
     right too, and costs another pass over the logits."""
-    return PolicyLoss(*_finetune.policy_loss(logits, choice, old_logp, advantage, ref_logp, mask, clip_low, clip_high, kl_coef, reduction, scale))
+    return PolicyLoss._make(_finetune.policy_loss(logits, choice, old_logp, advantage, ref_logp, mask, clip_low, clip_high, kl_coef, reduction, scale))
 
 
 def preference_loss(better: torch.Tensor, worse: torch.Tensor, better_ref: Optional[torch.Tensor] = None, worse_ref: Optional[torch.Tensor] = None, *,
@@ -78,7 +78,7 @@ def preference_loss(better: torch.Tensor, worse: torch.Tensor, better_ref: Optio
 
     averaged over the pairs or summed, times ``scale``.  The two sides may have different lengths (0 included); masked steps may hold anything and get a zero
     gradient.  Differentiable in ``better`` and ``worse`` (once); the sums are held in 64 bits."""
-    return PreferenceLoss(*_finetune.preference_loss(better, worse, better_ref, worse_ref, better_mask, worse_mask, beta, label_smoothing, reduction, scale))
+    return PreferenceLoss._make(_finetune.preference_loss(better, worse, better_ref, worse_ref, better_mask, worse_mask, beta, label_smoothing, reduction, scale))
 
 
 def clip_grads_(grads: Iterable[Optional[torch.Tensor]], max_norm: float, *, eps: float = 1e-6) -> torch.Tensor:
