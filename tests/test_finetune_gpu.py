@@ -496,6 +496,19 @@ def test_clip_grads(ft, dtype, sizes, max_norm):
             close(g, w * c, (w * c).abs() * (torch.finfo(dtype).eps / 2 + 3 * U) + (2.0 ** -25 if dtype == torch.float16 else 0.0), "scaled")
 
 
+def test_clip_grads_beyond_32_bits(ft):
+    """One tensor of more than 2^31 elements (a table takes 2^31 of a range at most), its values at both ends and around the seam."""
+    n = (1 << 31) + 12347
+    g = torch.zeros(n, dtype=torch.bfloat16, device=dev())
+    at = torch.tensor([0, 1, 4095, (1 << 31) - 1, 1 << 31, (1 << 31) + 1, n - 2, n - 1], device=dev())
+    g[at] = 3.0
+    other = torch.full((5,), 4.0, device=dev())
+    norm = math.sqrt(8 * 9.0 + 5 * 16.0)
+    assert float(ft.clip_grads_([g, other], 1.0)) == pytest.approx(norm, rel=1e-7)
+    assert (g[at].double() - 3.0 / norm).abs().max() < 3.0 / norm * 2.0 ** -8 and (other.double() - 4.0 / norm).abs().max() < 1e-6
+    assert int(torch.count_nonzero(g)) == 8
+
+
 def test_clip_grads_mixed_lists(ft):
     """Types mixed, views of one buffer at odd offsets, other orders of dimensions, None entries, neighbours left as they were."""
     flat = rand(100000, seed=5).to(dev())
