@@ -1001,7 +1001,7 @@ constexpr int kShort = 32;             // elements a row of k_rows_short may hav
 // lanes of a short row, four elements each: the fewest, because a wave pays the end of a row once for all the rows it has
 // (10^6 rows of 6 fp32 with gradient: 8 lanes of one element 69 us, 2 of four 26; of 30 bf16, forward: 32 of one 140 us, 8 of four 41)
 int short_lanes(int64_t k) { return k <= 4 ? 1 : k <= 8 ? 2 : k <= 16 ? 4 : 8; }
-RowPlan plan_rows(int64_t rows, int64_t k, int size) {
+RowPlan plan_rows(int64_t rows, int64_t k, int size, int mode) {
   const int64_t bytes = k * size, pieces = k * size / 16;
   RowPlan p{SHORT, 1, 1, k};
   auto grid = [&](int64_t per_block, int64_t most) { const int64_t b = (rows + per_block - 1) / per_block; return b < most ? b : most; };
@@ -1023,7 +1023,9 @@ RowPlan plan_rows(int64_t rows, int64_t k, int size) {
   } else if (pieces <= 512) {
     p.kind = HELD;
     p.grid = grid(pieces <= 64 ? 32 : pieces <= 128 ? 16 : pieces <= 256 ? 8 : 4, rows);
-  } else if (pieces <= 16384) {
+  } else if (pieces <= (mode == LOGP && rows > 128 ? 8192 : 16384)) {
+    // (with no gradient in view parts of rows overlap better than a block of 16 waves per CU: 131072 bf16, one block / parts, 2048 rows 111 / 88 us, 300 rows
+    // 25.7 / 21.5, 100 rows 12.0 / 13.9; shorter rows, 65536 bf16 x 4096: 85 / 90)
     p.kind = HELD;
     p.grid = rows;
   } else {
@@ -1082,9 +1084,9 @@ template <typename T, int MODE, int GRAD> void launch_rows(Launches& run, const 
 }
 
 // count | (loss, kl, clipped) per block | partial results of split rows | (maximum, 1 / sum) and coefficient of very long rows
-int64_t row_space(const ps_decisions* d) {
+int64_t row_space(const ps_decisions* d, int mode) {
   if (d->rows < 1 || d->choices < 1) return 8;
-  const RowPlan p = plan_rows(d->rows, d->choices, d->dtype == PS_F32 ? 4 : 2);
+  const RowPlan p = plan_rows(d->rows, d->choices, d->dtype == PS_F32 ? 4 : 2, mode);
   return 8 + 24 * p.parts(d->rows) + (p.kind == SPLIT || p.kind == VERY_LONG ? 16 * p.grid : 0) + (p.kind == VERY_LONG ? 12 * d->rows : 0);
 }
 struct RowSpace {
@@ -1102,20 +1104,24 @@ int check_space(const void* p, int64_t bytes, int64_t need, const char* what) {
 }
 }  // namespace
 
-extern "C" int64_t ps_choice_workspace(const ps_decisions* d) { return d ? row_space(d) : set_error(PS_E_ARG, "ps_choice_workspace: no decisions"); }
+extern "C" int64_t ps_choice_workspace(const ps_decisions* d) { 
+  if (!d) return set_error(PS_E_ARG, "ps_choice_workspace: no decisions");
+  const int64_t a = row_space(d, LOGP), b = row_space(d, POLICY);
+  return a > b ? a : b;
+}
 
 extern "C" int ps_choice_logp(const ps_decisions* d, float* logp, float* stat, void* workspace, int64_t workspace_bytes, void* stream) {
   RowIo io{};
   if (int e = check_rows(d, "ps_choice_logp", &io.r)) return e;
   if (!io.r.rows) return PS_OK;
   if (!logp || ((uintptr_t)stat & 7)) return set_error(PS_E_ARG, "ps_choice_logp: NULL logp, or stat is not aligned");
-  if (int e = check_space(workspace, workspace_bytes, row_space(d), "ps_choice_logp")) return e;
+  if (int e = check_space(workspace, workspace_bytes, row_space(d, LOGP), "ps_choice_logp")) return e;
   Launches run{(hipStream_t)stream};
   io.logp = logp;
   io.stat = (float2*)stat;
   by_type(d->dtype, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
-    const RowPlan p = plan_rows(io.r.rows, io.r.k, sizeof(T));
+    const RowPlan p = plan_rows(io.r.rows, io.r.k, sizeof(T), LOGP);
     launch_rows<T, LOGP, GRAD_NONE>(run, io, p, RowSpace(workspace, p, io.r.rows).parts);
     return 0;
   });
@@ -1148,9 +1154,9 @@ extern "C" int ps_policy_loss(const ps_decisions* d, const ps_policy_terms* q, f
   if (!std::isfinite(q->scale)) return set_error(PS_E_ARG, "ps_policy_loss: scale must be finite");
   if (q->kl_coef > 0.0 && !q->ref_logp && r.rows) return set_error(PS_E_ARG, "ps_policy_loss: kl_coef without ref_logp");
   if (((uintptr_t)grad & (d->dtype == PS_F32 ? 3 : 1)) || ((uintptr_t)stat & 7)) return set_error(PS_E_ARG, "ps_policy_loss: grad or stat is not aligned");
-  if (int e = check_space(workspace, workspace_bytes, row_space(d), "ps_policy_loss")) return e;
+  if (int e = check_space(workspace, workspace_bytes, row_space(d, POLICY), "ps_policy_loss")) return e;
   Launches run{(hipStream_t)stream};
-  const RowPlan p = r.rows ? plan_rows(r.rows, r.k, d->dtype == PS_F32 ? 4 : 2) : RowPlan{SHORT, 0, 1, 0};
+  const RowPlan p = r.rows ? plan_rows(r.rows, r.k, d->dtype == PS_F32 ? 4 : 2, POLICY) : RowPlan{SHORT, 0, 1, 0};
   const RowSpace w(workspace, p, r.rows);
   // the valid rows of a short mask are counted by every block for itself (1 - 2 us, all at once where the blocks are few), else by a launch (5 us)
   const bool counted = r.mask && (r.rows > 16384 || p.grid > 1024);

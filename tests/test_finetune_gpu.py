@@ -72,7 +72,7 @@ def close(got, want, tol, what=""):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() - tol)[bad].max())} beyond its bound"
 
 
-ROWS_CHOICES = [(40000, 30), (30000, 4), (257, 5), (9000, 8), (1000, 9), (7000, 16), (70, 250), (90, 600), (60, 2048), (1, 1), (5, 1), (1, 2), (3, 3), (1025, 3), (17, 7), (64, 16), (65, 17), (31, 64), (33, 65), (9, 127), (10, 128), (7, 255), (5, 257), (130, 511), (4, 513),
+ROWS_CHOICES = [(130, 70001), (129, 131080), (40000, 30), (30000, 4), (257, 5), (9000, 8), (1000, 9), (7000, 16), (70, 250), (90, 600), (60, 2048), (1, 1), (5, 1), (1, 2), (3, 3), (1025, 3), (17, 7), (64, 16), (65, 17), (31, 64), (33, 65), (9, 127), (10, 128), (7, 255), (5, 257), (130, 511), (4, 513),
                 (3, 1000), (6, 1024), (5, 2049), (2, 4096), (3, 4099), (2, 8191), (3, 16387), (2, 32768), (1, 50021), (2, 65537), (1, 131072), (2, 131071), (1, 200003),
                 (300, 1111), (2500, 40), (70, 9001)]
 
