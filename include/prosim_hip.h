@@ -332,7 +332,7 @@ int32_t ps_num_map_tokens(ps_engine* e);
  * choice (ps_set_mode_choice's table, or a token of a motion vocabulary), two losses over it, and the clipping of the gradients.  They need no
  * engine: every pointer is a DEVICE pointer unless it says HOST, everything is enqueued on `stream` (a hipStream_t, NULL = the default
  * stream; the stream's device must be the current one), nothing is synchronised, allocated or kept between calls, and every call can be
- * captured into a graph.  Results depend on the inputs alone (no atomics): equal inputs give equal bits.  Workspaces belong to one call at
+ * captured into a graph.  There are no atomics: equal inputs at equally aligned addresses give equal bits.  Workspaces belong to one call at
  * a time, need no initialisation and are 8-byte aligned, `stat` too; outputs overlap neither inputs nor each other. */
 #define PS_F32 0
 #define PS_BF16 1

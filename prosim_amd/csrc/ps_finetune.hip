@@ -3,7 +3,8 @@
 //
 // All of them move bytes: ~10 operations per element against 2 - 8 B of HBM traffic, so what is designed for is one pass over the data.
 // Statistics (sums of exponentials, log-probabilities, squares, losses) are held in 64 bits; only elements and stored results are narrower.
-// No atomics: every sum has an order that depends on sizes alone, so equal inputs return equal bits.
+// No atomics: every sum has an order that depends on sizes, types and the alignment of addresses alone (a gradient list's on which tensors are neighbours
+// as well), so a call repeats its bits.
 #include "prosim_hip.h"
 
 #include <hip/hip_runtime.h>

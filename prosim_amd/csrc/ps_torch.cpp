@@ -288,22 +288,26 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& better, const Tensor& w
 bool dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
 Tensor clip_grads(const py::list& list, double max_norm, double eps) {
-  std::vector<Tensor> ts;
+  std::vector<const Tensor*> ts;      // (the list keeps them)
   ts.reserve(list.size());
-  for (const py::handle h : list) {
-    if (h.is_none()) continue;
-    TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), "grads: expected tensors, got ", Py_TYPE(h.ptr())->tp_name);
-    ts.push_back(THPVariable_Unpack(h.ptr()));
+  for (Py_ssize_t i = 0, n = PyList_GET_SIZE(list.ptr()); i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(list.ptr(), i);
+    if (o == Py_None) continue;
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "grads: expected tensors, got ", Py_TYPE(o)->tp_name);
+    ts.push_back(&THPVariable_Unpack(o));
   }
   TORCH_CHECK_VALUE(!ts.empty(), "clip_grads_: no gradients");
+  const Tensor& like = *ts[0];
+  check_gpu(like, "grads");
   // Ranges of memory, by address: that finds tensors on top of each other, and makes one range of neighbours -- data-parallel training keeps its
   // gradients as views of a few flat buffers, hundreds of tensors that are then a handful of ranges.
   struct Range { uintptr_t begin, end; int32_t dtype; };
   std::vector<Range> used;
   used.reserve(ts.size());
   bool sorted = true;
-  for (const Tensor& t : ts) {
-    check_gpu(t, "grads", ts[0]);
+  for (const Tensor* p : ts) {
+    const Tensor& t = *p;
+    if (t.device() != like.device() || t.layout() != at::kStrided) check_gpu(t, "grads", like);
     const int dtype = dtype_of(t);
     TORCH_CHECK_TYPE(dtype >= 0, "grads: expected float32, bfloat16 or float16, got ", type_name(t));
     TORCH_CHECK_VALUE(!t.requires_grad(), "grads: a tensor requires a gradient itself (parameters instead of their gradients?)");
@@ -330,11 +334,11 @@ Tensor clip_grads(const py::list& list, double max_norm, double eps) {
     }
   }
   const int32_t n = (int32_t)at.size();
-  const c10::DeviceGuard guard(ts[0].device());
-  const Tensor norm = empty({}, ts[0]), space = empty({ps_clip_grads_workspace(n, numel.data(), dtypes.data())}, ts[0], at::kByte);
-  check(ps_clip_grads(n, at.data(), numel.data(), dtypes.data(), max_norm, eps, ptr<float>(norm), space.data_ptr(), space.numel(), stream_of(ts[0])));
-  for (const Tensor& t : ts)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  const c10::DeviceGuard guard(like.device());
+  const Tensor norm = empty({}, like), space = empty({ps_clip_grads_workspace(n, numel.data(), dtypes.data())}, like, at::kByte);
+  check(ps_clip_grads(n, at.data(), numel.data(), dtypes.data(), max_norm, eps, ptr<float>(norm), space.data_ptr(), space.numel(), stream_of(like)));
+  for (const Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 }  // namespace

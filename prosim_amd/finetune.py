@@ -10,7 +10,7 @@ vocabulary.  The engine rolls out (``Engine.set_replicas`` gives M rollouts of a
 Plain tensors on the GPU in, tensors out (HIP kernels behind the C ABI of include/prosim_hip.h; no CPU fallback).  Everything is enqueued on torch's
 current stream of the tensors' device -- ``torch.cuda.ExternalStream(engine.stream_handle)`` orders it behind an engine's rollout -- nothing
 synchronises, every call may be captured into a graph (with ``torch.autograd.grad``; as always in torch, no eager graph of the same leaves may be alive
-while a backward pass is captured), and equal inputs give equal bits.  Wrong arguments raise TypeError / ValueError before anything is launched.
+while a backward pass is captured), and equal inputs at equally aligned addresses give equal bits.  Wrong arguments raise TypeError / ValueError before anything is launched.
 """
 from __future__ import annotations
 
