@@ -27,11 +27,21 @@ template <typename T> __device__ __forceinline__ float to_f32(T v) { return (flo
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }   // (round to nearest even, once per stored element)
 
 // e^d for d <= 0.  fp32 elements take the library's expf (their results keep 24 bits); 16-bit elements v_exp_f32 on d * log2(e), the constant
-// in two parts (in one, its error would move every term of a sum the same way): what is left is the product's rounding, |d| 2^-24 relative.
+// in two parts (in one, its error would move every term of a sum the same way), the small one first: behind the rounded product it is less than half a
+// step and would be lost.  What is left is one rounding, |d| 2^-24 relative.
 template <typename T> __device__ __forceinline__ float exp_of(float d) {
-  return __builtin_amdgcn_exp2f(fmaf(d, 1.92596299e-8f, d * 1.44269502e+0f));
+  return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502e+0f, d * 1.92596299e-8f));
 }
 template <> __device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
+// Sum of N of them, each added in 64 bits: 32-bit partial sums of four to eight terms would cost a log-probability as much again as its own rounding
+// (2048 rows of 4 in fp32: 4.4e-8 against 2.4e-8 rms) and save nothing, the additions hide behind the loads (2048 x 32768 bf16 53.5 us both ways, 65536 x
+// 2048 fp32 190 us both ways).
+template <typename T, int N> __device__ __forceinline__ double sum_of_exp(const float* f, float base) {
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) s += (double)exp_of<T>(f[j] - base);
+  return s;
+}
 
 // The few 64-bit functions a row needs at its end, to about 1e-11 relative -- far beyond what its sum of exponentials carries -- in a quarter of the
 // library's instructions (a wave spends as long on the library's log, exp and expm1 as on 1500 elements) and without its 40 registers of constants.
@@ -354,13 +364,12 @@ template <typename T, int G, int N, int MODE, int GRAD> __global__ void __launch
     }
     a.m = wave_max<G>(a.m);
     const float base = base_of(a.m);
-    float t = 0.0f;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       f[q] = exp_of<T>(f[q] - base);
-      t += f[q];
+      a.s += (double)f[q];
     }
-    a.s = wave_sum<G>((double)t);
+    a.s = wave_sum<G>(a.s);
     const RowEnd e = end_row<MODE>(io, i, terms, ok, xc, a, weight, lane == 0, acc);
     if (GRAD) {
       const float scale = -e.coef * e.inv;
@@ -479,12 +488,10 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
 #pragma unroll
       for (int q = 0; q < NV; ++q)
         if (q * TPR + t < nv) {
-          float f[V], e = 0.0f;
+          float f[V];
           v[q].forget();
           v[q].get(f);
-#pragma unroll
-          for (int j = 0; j < V; ++j) e += exp_of<T>(f[j] - base);
-          a.s += (double)e;          // (eight terms in 32 bits, then 64)
+          a.s += sum_of_exp<T, V>(f, base);
           __builtin_amdgcn_sched_barrier(0);
         }
       a.s = wave_sum<LANES>(a.s);
@@ -549,12 +556,10 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (q + u * THREADS < n) {
-        float f[V], e = 0.0f;
+        float f[V];
         v[u].forget();
         v[u].get(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) e += exp_of<T>(f[j] - base);
-        a.s += (double)e;
+        a.s += sum_of_exp<T, V>(f, base);
       }
   }
   if ((int)threadIdx.x < sh.edges) {
