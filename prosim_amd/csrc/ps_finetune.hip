@@ -33,13 +33,18 @@ template <typename T> __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502e+0f, d * 1.92596299e-8f));
 }
 template <> __device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
-// Sum of N of them, each added in 64 bits: 32-bit partial sums of four to eight terms would cost a log-probability as much again as its own rounding
-// (2048 rows of 4 in fp32: 4.4e-8 against 2.4e-8 rms) and save nothing, the additions hide behind the loads (2048 x 32768 bf16 53.5 us both ways, 65536 x
-// 2048 fp32 190 us both ways).
-template <typename T, int N> __device__ __forceinline__ double sum_of_exp(const float* f, float base) {
+// Sum of N of them in 64 bits, TERMS at a time: single ones in rows that less than a wave holds, where 32-bit partial sums of four to eight terms would
+// cost a log-probability as much again as its own rounding (8192 x 64 fp32: 4.3e-8 against 2.8e-8 rms); pairs in longer rows, where a pair's rounding is
+// lost among those of the exponentials and half the conversions are measurable (3001 x 50021 fp16: 57 us singly, 55 us in pairs, 54 us eight at a time;
+// 2048 x 131072 bf16 with its gradient 217, 210, 207 us).
+template <typename T, int N, int TERMS> __device__ __forceinline__ double sum_of_exp(const float* f, float base) {
   double s = 0.0;
 #pragma unroll
-  for (int j = 0; j < N; ++j) s += (double)exp_of<T>(f[j] - base);
+  for (int j = 0; j < N; j += TERMS) {
+    float e = exp_of<T>(f[j] - base);
+    if (TERMS == 2) e += exp_of<T>(f[j + 1] - base);
+    s += (double)e;
+  }
   return s;
 }
 
@@ -491,7 +496,7 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
           float f[V];
           v[q].forget();
           v[q].get(f);
-          a.s += sum_of_exp<T, V>(f, base);
+          a.s += sum_of_exp<T, V, TPR < 64 ? 1 : 2>(f, base);
           __builtin_amdgcn_sched_barrier(0);
         }
       a.s = wave_sum<LANES>(a.s);
@@ -559,7 +564,7 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
         float f[V];
         v[u].forget();
         v[u].get(f);
-        a.s += sum_of_exp<T, V>(f, base);
+        a.s += sum_of_exp<T, V, 2>(f, base);
       }
   }
   if ((int)threadIdx.x < sh.edges) {

@@ -2,8 +2,9 @@
 
 Tolerances, with u = 2^-24 (half a step of float32):
 * an exponential e^d, d = x - max <= 0, is off by at most (|d| + |d| / 2 + 2) u * 2 relative (rounding of d, of its product with log2 e and of that
-  constant, one step of the exponential); a row's sum is added in 64 bits.  Weighted with p = e^d / s, sum p |d| = H - ln s <= ln K, so ln s is off by
-  at most u (3 ln K + 4), and a stored log-probability by u (|logp| + 3 ln K + 4); the end of a row (its 64-bit logarithm) is far below the 4 u left.
+  constant, one step of the exponential); a row's sum adds at most two terms in
+  float32 before it goes to 64 bits (1 u).  Weighted with p = e^d / s, sum p |d| = H - ln s <= ln K, so ln s is off by
+  at most u (3 ln K + 5), and a stored log-probability by u (|logp| + 3 ln K + 5); the end of a row (its 64-bit logarithm) is far below the 3 u left.
 * a gradient element coef (one-hot - p): half a step of its type, plus |coef| p u (3 |d| + 8 + the sum's error) and the one-hot difference's 2 u |coef|,
   plus the error of coef: its own rounding and the log-probability's error times d coef / d logp.
 """
