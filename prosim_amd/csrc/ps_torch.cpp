@@ -24,9 +24,14 @@ typedef std::optional<Tensor> Maybe;
 
 const char* type_name(const Tensor& t) { return c10::toString(t.scalar_type()); }
 
+// Is the tensor's memory what the tensor says?  (the imaginary part of a conjugate is a view whose sign is a flag; torch's efficient zeros have no memory)
+bool as_stored(const Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
 void check_gpu(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda() && t.layout() == at::kStrided, name, ": expected a dense tensor on the GPU, got one on ", t.device(), " (", t.layout(), ")");
+  TORCH_CHECK_VALUE(as_stored(t), name, ": a lazily negated or zero tensor: clone() it");
 }
+// an incoming gradient as dense memory
+Tensor incoming(const Tensor& g) { return (as_stored(g) ? g : g.clone()).contiguous(); }
 void check_gpu(const Tensor& t, const char* name, const Tensor& like) {
   check_gpu(t, name);
   TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", the other tensors are on ", like.device());
@@ -165,7 +170,7 @@ struct ChoiceLogp : torch::autograd::Function<ChoiceLogp> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
-    const Tensor coef = grads[0].contiguous();
+    const Tensor coef = incoming(grads[0]);
     const int64_t n = s[1].numel();
     return once({choice_grad(s[0], s[1], s[2], (float*)((char*)s[3].data_ptr() + s[3].numel() - 12 * n), ptr<float>(coef), nullptr, Tensor()), Tensor()});
   }
@@ -208,7 +213,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
       ready = it->second.toTensor();
       ctx->saved_data.erase(it);
     }
-    const Tensor gain = grads[0].contiguous();
+    const Tensor gain = incoming(grads[0]);
     const int64_t n = s[1].numel();
     const float* stat = (float*)((char*)s[3].data_ptr() + s[3].numel() - 12 * n);
     return once({choice_grad(s[0], s[1], s[2], stat, stat + 2 * n, ptr<float>(gain), ready), Tensor(), Tensor()});
@@ -261,7 +266,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     q.pairs = pairs;
     q.better_steps = shapes[1] < 0 ? 1 : shapes[1];
     q.worse_steps = shapes[2] < 0 ? 1 : shapes[2];
-    const Tensor gain = grads[0].contiguous();
+    const Tensor gain = incoming(grads[0]);
     check(ps_preference_grad(&q, (float*)((char*)s[0].data_ptr() + s[0].numel() - 4 * pairs), ptr<float>(gain), ptr<float>(out[0]), ptr<float>(out[1]), stream_of(s[0])));
     return once({out[0], out[1], Tensor(), Tensor(), Tensor()});
   }
@@ -307,7 +312,7 @@ Tensor clip_grads(const py::list& list, double max_norm, double eps) {
   bool sorted = true;
   for (const Tensor* p : ts) {
     const Tensor& t = *p;
-    if (t.device() != like.device() || t.layout() != at::kStrided) check_gpu(t, "grads", like);
+    if (t.device() != like.device() || t.layout() != at::kStrided || !as_stored(t)) check_gpu(t, "grads", like);
     const int dtype = dtype_of(t);
     TORCH_CHECK_TYPE(dtype >= 0, "grads: expected float32, bfloat16 or float16, got ", type_name(t));
     TORCH_CHECK_VALUE(!t.requires_grad(), "grads: a tensor requires a gradient itself (parameters instead of their gradients?)");

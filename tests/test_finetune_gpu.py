@@ -598,6 +598,27 @@ def test_refusals(ft):
     assert y is not None
 
 
+def test_tensors_whose_memory_is_not_their_value(ft):
+    """The imaginary part of a conjugate is a view with a flag for its sign, torch's efficient zeros have no memory: refused as inputs, right as incoming
+    gradients."""
+    x, c, f = rand(6, 5, seed=4).to(dev()), torch.arange(6, device=dev()) % 5, rand(6, seed=5).to(dev())
+    neg = lambda t: torch.complex(t, -t).conj().imag          # = t
+    zero = lambda *s: torch._efficientzerotensor(s, device=dev(), dtype=torch.float32)
+    assert neg(x).is_neg() and zero(6)._is_zerotensor()
+    for bad in (lambda: ft.choice_logp(neg(x), c), lambda: ft.choice_logp(zero(6, 5), c), lambda: ft.policy_loss(x, c, neg(f), f), lambda: ft.policy_loss(x, c, f, zero(6)),
+                lambda: ft.policy_loss(x, c, f, f, ref_logp=zero(6)), lambda: ft.preference_loss(f, neg(f)), lambda: ft.preference_loss(f, f, zero(6)), lambda: ft.clip_grads_([f, neg(x)], 1.0),
+                lambda: ft.clip_grads_([zero(6)], 1.0)):
+        with pytest.raises(ValueError):
+            bad()
+    a, b = x.clone().requires_grad_(True), f.clone().requires_grad_(True)
+    one = torch.full((), 0.75, device=dev())
+    for out, leaf, g, none in ((lambda: ft.choice_logp(a, c), a, f, zero(6)), (lambda: ft.policy_loss(a, c, f, f).loss, a, one, zero()), (lambda: ft.preference_loss(b, f * 2).loss, b, one, zero())):
+        want, = torch.autograd.grad(out(), leaf, g)
+        got, = torch.autograd.grad(out(), leaf, neg(g))
+        assert torch.equal(got, want) and want.abs().max() > 0
+        assert (torch.autograd.grad(out(), leaf, none)[0] == 0).all()
+
+
 def test_calls_from_several_threads(ft):
     """Four host threads, each on a stream of its own, at once."""
     from concurrent.futures import ThreadPoolExecutor
