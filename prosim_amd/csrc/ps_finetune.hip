@@ -33,19 +33,17 @@ template <typename T> __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502e+0f, d * 1.92596299e-8f));
 }
 template <> __device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
-// Sum of N of them in 64 bits, TERMS at a time: single ones in rows that less than a wave holds, where 32-bit partial sums of four to eight terms would
-// cost a log-probability as much again as its own rounding (8192 x 64 fp32: 4.3e-8 against 2.8e-8 rms); pairs in longer rows, where a pair's rounding is
-// lost among those of the exponentials and half the conversions are measurable (3001 x 50021 fp16: 57 us singly, 55 us in pairs, 54 us eight at a time;
-// 2048 x 131072 bf16 with its gradient 217, 210, 207 us).
-template <typename T, int N, int TERMS> __device__ __forceinline__ double sum_of_exp(const float* f, float base) {
-  double s = 0.0;
+// The same in long rows, element j of a 16-byte piece: the product with log2(e) is rounded once, by a constant whose error is 1.3e-8 below in seven elements
+// and 6.9e-8 above in the eighth -- together 0.3e-8, so a sum over many carries none of it worth naming, and each element less than its rounding.
+template <typename T> __device__ __forceinline__ float exp_of(float d, int j) {
+  return sizeof(T) == 4 ? exp_of<T>(d) : __builtin_amdgcn_exp2f(d * (j == 0 ? 1.44269514e+0f : 1.44269502e+0f));
+}
+
+// s += N of them, each added in 64 bits: 32-bit partial sums lose as much as a result's own rounding where one element carries the row (log-probabilities of
+// 8192 x 64 fp32: 4.3e-8 against 2.8e-8 rms in sums of four; 2048 x 131072 bf16: 3.5e-8 against 2.9e-8 even in pairs, which would save 2 % of its time, 7 % of 3001 x 50021 fp16).
+template <typename T, int N, bool LONG> __device__ __forceinline__ void add_exp(double& s, const float* f, float base) {
 #pragma unroll
-  for (int j = 0; j < N; j += TERMS) {
-    float e = exp_of<T>(f[j] - base);
-    if (TERMS == 2) e += exp_of<T>(f[j + 1] - base);
-    s += (double)e;
-  }
-  return s;
+  for (int j = 0; j < N; ++j) s += (double)(LONG ? exp_of<T>(f[j] - base, j) : exp_of<T>(f[j] - base));
 }
 
 // The few 64-bit functions a row needs at its end, to about 1e-11 relative -- far beyond what its sum of exponentials carries -- in a quarter of the
@@ -131,8 +129,11 @@ struct Rows {
   const uint8_t* mask;    // per row, or NULL
   int choice64;
 };
+// (no branch on the type: its arithmetic would wait for the load where it stands)
 __device__ __forceinline__ int64_t choice_of(const Rows& r, int64_t i) {
-  return r.choice64 ? ((const int64_t*)r.choice)[i] : (int64_t)((const int32_t*)r.choice)[i];
+  const int32_t* p = (const int32_t*)r.choice + (i << r.choice64);
+  const int32_t low = p[0], high = p[r.choice64];
+  return r.choice64 ? (int64_t)high << 32 | (uint32_t)low : (int64_t)low;
 }
 
 struct Policy {
@@ -210,6 +211,7 @@ template <typename T> struct Reg {
   // the packed words are what lives from one use to the next: without this the compiler keeps the 32-bit elements of the first use (twice the
   // registers, 128 - 2000 B of scratch per lane in the widest kernels)
   __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])); }
+  __device__ __forceinline__ float top(float m) const;      // max(m, the elements)
   __device__ __forceinline__ void get(float* f) const;
   __device__ __forceinline__ void set(const float* f);
 };
@@ -252,6 +254,33 @@ template <> __device__ __forceinline__ void Reg<f16>::get(float* f) const {
 template <> __device__ __forceinline__ void Reg<f16>::set(const float* f) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = pack2<f16>(f[2 * i], f[2 * i + 1]);
+}
+// The running maximum: fp16 two elements at a time without unpacking them (6 operations a piece instead of 12; with one rounding of the exponent's product
+// less this took 3001 x 50021 fp16 from 57 to 54 us: two blocks of 8 waves share a CU's registers there, and their arithmetic, about 50 cycles an element and
+// SIMD, 16 of them the exponential, is not all hidden behind each other's loads).  A NaN may be taken or passed
+// over; the row's sum has it either way.  A bf16 word must not stand for its upper element as it is: -inf with bits behind it is a signalling NaN, which
+// v_max_f32 answers with a NaN; and packed integer maxima for both signs took 65 us instead of 63.
+template <> __device__ __forceinline__ float Reg<float>::top(float m) const {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, __uint_as_float(w[i]));
+  return m;
+}
+template <> __device__ __forceinline__ float Reg<bf16>::top(float m) const {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = fmaxf(fmaxf(m, __uint_as_float(w[i] << 16)), __uint_as_float(w[i] & 0xffff0000u));
+  return m;
+}
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("v_pk_max_f16 %0, %1, %2" : "=v"(m) : "v"(a), "v"(b));      // (the builtin quiets both operands first, three instructions for one)
+  return m;
+}
+template <> __device__ __forceinline__ float Reg<f16>::top(float m) const {
+  typedef f16 h2 __attribute__((ext_vector_type(2)));
+  const uint32_t a = pk_max(pk_max(w[0], w[1]), pk_max(w[2], w[3]));
+  h2 h;
+  __builtin_memcpy(&h, &a, 4);
+  return fmaxf(fmaxf(m, (float)h.x), (float)h.y);
 }
 
 // (maximum, sum of exponentials relative to it) of a part of a row.  A part of -inf alone keeps the maximum -inf and the sum 0.
@@ -462,32 +491,28 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
   const int64_t i = block * (THREADS / TPR) + (TPR < 64 ? (int)threadIdx.x / TPR : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR));
   if (i < r.rows) {
     T* dx = GRAD ? (T*)io.dx + i * r.k : nullptr;
+    const int64_t c = choice_of(r, i);        // (beside the mask's byte and before the row: the chosen logit's address waits for nothing else)
     if (r.mask && !r.mask[i]) {        // (the same for all of the row's threads)
       if (t == 0) masked_row(io, i);
       if (GRAD) zero_row<T, TPR>(dx, r.k, t);
     } else {
       const T* x = (const T*)r.x + i * r.stride;
-      const int64_t c = choice_of(r, i);        // (the first load: the chosen logit's address waits for nothing else)
       const Shared<T, TPR> sh(x, r.k);
       const int nv = sh.pieces;
       Reg<T> v[NV];
 #pragma unroll
       for (int q = 0; q < NV; ++q)
         if (q * TPR + t < nv) v[q].load_once(x + sh.head + q * (TPR * V) + (uint32_t)(t * V));
-      const float last = t < sh.edges ? to_f32(x[sh.edge(t)]) : -INFINITY;
+      const T end = x[t < sh.edges ? sh.edge(t) : 0];      // (in every thread: converted where only some have one, it would wait for the whole row)
       const bool ok = c >= 0 && c < r.k;
       const float xc = to_f32(x[ok ? c : 0]);
       const RowTerms terms = MODE == POLICY ? terms_of(io.p, i) : RowTerms{};
-      Part a{0.0, last};
+      Part a{0.0, -INFINITY};
 #pragma unroll
       for (int q = 0; q < NV; ++q)
-        if (q * TPR + t < nv) {
-          float f[V];
-          v[q].get(f);
-#pragma unroll
-          for (int j = 0; j < V; ++j) a.m = fmaxf(a.m, f[j]);
-        }
-      a.m = wave_max<LANES>(a.m);
+        if (q * TPR + t < nv) a.m = v[q].top(a.m);
+      const float last = t < sh.edges ? to_f32(end) : -INFINITY;
+      a.m = wave_max<LANES>(fmaxf(a.m, last));
       const float base = base_of(a.m);
       a.s = (double)exp_of<T>(last - base);
 #pragma unroll
@@ -496,7 +521,7 @@ template <typename T, int TPR, int NV, int MODE, int GRAD> __global__ void __lau
           float f[V];
           v[q].forget();
           v[q].get(f);
-          a.s += sum_of_exp<T, V, TPR < 64 ? 1 : 2>(f, base);
+          add_exp<T, V, TPR >= 64>(a.s, f, base);
           __builtin_amdgcn_sched_barrier(0);
         }
       a.s = wave_sum<LANES>(a.s);
@@ -550,12 +575,7 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (q + u * THREADS < n) {
-        float f[V];
-        v[u].get(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) m = fmaxf(m, f[j]);
-      }
+      if (q + u * THREADS < n) m = v[u].top(m);
     raise(m);
     const float base = base_of(a.m);
 #pragma unroll
@@ -564,7 +584,7 @@ template <typename T, int THREADS> __device__ __forceinline__ Part stream_part(c
         float f[V];
         v[u].forget();
         v[u].get(f);
-        a.s += sum_of_exp<T, V, 2>(f, base);
+        add_exp<T, V, true>(a.s, f, base);
       }
   }
   if ((int)threadIdx.x < sh.edges) {

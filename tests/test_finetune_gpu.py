@@ -2,9 +2,9 @@
 
 Tolerances, with u = 2^-24 (half a step of float32):
 * an exponential e^d, d = x - max <= 0, is off by at most (|d| + |d| / 2 + 2) u * 2 relative (rounding of d, of its product with log2 e and of that
-  constant, one step of the exponential); a row's sum adds at most two terms in
-  float32 before it goes to 64 bits (1 u).  Weighted with p = e^d / s, sum p |d| = H - ln s <= ln K, so ln s is off by
-  at most u (3 ln K + 5), and a stored log-probability by u (|logp| + 3 ln K + 5); the end of a row (its 64-bit logarithm) is far below the 3 u left.
+  constant, one step of the exponential); a row's sum is added in 64 bits.
+  Weighted with p = e^d / s, sum p |d| = H - ln s <= ln K, so ln s is off by at most u (3 ln K + 4), and a stored log-probability by
+  u (|logp| + 3 ln K + 4); the end of a row (its 64-bit logarithm) is far below the 4 u left.
 * a gradient element coef (one-hot - p): half a step of its type, plus |coef| p u (3 |d| + 8 + the sum's error) and the one-hot difference's 2 u |coef|,
   plus the error of coef: its own rounding and the log-probability's error times d coef / d logp.
 """
@@ -282,6 +282,21 @@ def test_the_mean_counts_valid_rows_in_every_layout(ft, rows, k):
     assert torch.equal(a.loss, b.loss) and torch.equal(a.logp, b.logp)
 
 
+@pytest.mark.parametrize("rows", [1, 15, 33, 5000, 16401, 70003])
+@pytest.mark.parametrize("off", [1, 3, 16])
+def test_a_mask_at_any_address(ft, rows, off):
+    x, c, old, adv, ref = policy_inputs(rows, 9, torch.bfloat16, seed=8)
+    mask = (torch.rand(off + rows + 64, generator=torch.Generator().manual_seed(rows)).to(dev()) < 0.5)      # (valid and masked bytes around it, too)
+    check_policy(ft, x, c, old, adv, ref, mask[off:off + rows], 0.1, "mean", 1.0)
+    steps = rows // 3
+    if steps:
+        m = mask[off:off + 3 * steps].view(3, steps)
+        w = rand(3, steps, seed=9).to(dev()).requires_grad_(True)
+        a, b = ft.preference_loss(w, w * 0.5, better_mask=m, worse_mask=m), ft.preference_loss(w, w * 0.5, better_mask=m.clone(), worse_mask=m.clone())
+        assert torch.equal(a.loss, b.loss) and torch.equal(a.margin, b.margin)
+        assert torch.equal(torch.autograd.grad(a.loss, w)[0], torch.autograd.grad(b.loss, w)[0])
+
+
 def test_mean_loss_of_many_rows_counts_its_mask(ft):
     rows, k = 70001, 6
     x, c, old, adv, ref = policy_inputs(rows, k, torch.float32, seed=3)
@@ -396,6 +411,38 @@ def test_infinities_and_bad_choices(ft, dtype, k):
     assert p.loss.isnan()
     gp, = torch.autograd.grad(p.loss, leaf)
     assert gp[5:7].isnan().all() and torch.isfinite(gp[[0, 1, 7]]).all() and (gp[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("k", [24, 300, 3000, 9001, 70001])
+def test_infinities_at_every_place_of_a_piece(ft, dtype, k):
+    """One special element per row, at 20 neighbouring columns in turn (both halves of a word, pieces' borders, the row's ends): +inf and NaN make the row
+    and its gradient NaN, -inf is a choice that cannot be drawn, the type's lowest value is one that never is."""
+    n = 20
+    cols = torch.cat([torch.arange(n), torch.arange(k - n, k)]).to(dev())
+    base, c = rand(2 * n, k, seed=12).to(dtype).to(dev()), (cols + 1) % k
+    at = torch.arange(2 * n, device=base.device)
+    for value in (math.inf, math.nan, -math.inf, torch.finfo(dtype).min):
+        x = base.clone()
+        x[at, cols] = value
+        leaf = x.clone().requires_grad_(True)
+        logp = ft.choice_logp(leaf, c)
+        grad, = torch.autograd.grad(logp.sum(), leaf)
+        if value in (-math.inf, torch.finfo(dtype).min):
+            want = plain_logp(x, c)
+            close(logp.detach(), want, U * want.abs() + row_slack(k))
+            coef = torch.ones(2 * n, device=base.device)
+            close(grad, plain_grad(x, c, coef), grad_tol(x, c, coef, torch.zeros_like(coef, dtype=torch.float64), dtype))
+            assert (grad[at, cols] == 0).all()
+        else:
+            assert logp.isnan().all() and grad.isnan().all()
+    x = torch.full((4, k), -math.inf, dtype=dtype, device=base.device)        # the type's lowest value everywhere; -inf everywhere; one element that is left
+    x[0] = torch.finfo(dtype).min
+    x[2, k // 2] = torch.finfo(dtype).min
+    x[3, 1] = torch.finfo(dtype).max
+    c = torch.tensor([k - 1, 0, k // 2, 1], device=base.device)
+    logp = ft.choice_logp(x, c)
+    assert abs(float(logp[0]) + math.log(k)) <= U * (math.log(k) + 8) and bool(logp[1].isnan()) and float(logp[2]) == 0.0 and float(logp[3]) == 0.0
 
 
 def test_layouts_and_shapes(ft):
